@@ -65,6 +65,8 @@ int trb200_device_arch(void);
  * backend for. */
 #define TRB200_DTYPE_F16 0
 #define TRB200_DTYPE_BF16 1
+#define TRB200_DTYPE_F32 2      /* logits of the token losses, gradients of AdamW */
+#define TRB200_DTYPE_NONE (-1)  /* AdamW: no 16-bit working copy */
 
 typedef struct trb200_conv_desc {
     int32_t n, h, w, c;          /* input activation X  [n,h,w,c]            */
@@ -314,6 +316,60 @@ int trb200_softmax_ce_fused_dtype(const void* logits, int64_t logits_stride, con
                                   int32_t batch, int32_t classes, int32_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* Losses over the log-probabilities of chosen classes, beside softmax-CE.    */
+/* The reference has no counterpart.  `logits` and `dlogits` are rows of      */
+/* `classes` elements of `dtype` (half, bfloat16 or float) with row strides   */
+/* in elements, aligned to their element only; dlogits must not overlap       */
+/* logits (not even in the padding between rows).  `scaling` is the loss scale */
+/* (device scalar): it multiplies dlogits, not the loss.                      */
+/* A row does not count if its label lies outside [0, classes), if its weight */
+/* is 0 or if all its logits are minus infinity: it adds nothing to the loss, */
+/* its row of dlogits is zero, and in the first two cases its logits are not  */
+/* read (they may hold anything).  rows may be 0.  Results are bitwise        */
+/* reproducible.                                                              */
+/* ------------------------------------------------------------------------- */
+
+/* logp[i] = z_i[y_i] - lse[i], lse[i] = log(sum_c exp(z_i[c])): what the policy that
+ * acted and the reference policy contribute to the losses below.  Label outside
+ * [0, classes): 0 and 0; all logits minus infinity: -inf and -inf.  lse may be NULL. */
+int trb200_token_logp(const void* logits, int64_t logits_stride, const int32_t* labels, float* logp, float* lse,
+                      int32_t rows, int32_t classes, int32_t dtype, void* stream);
+
+/* Clipped policy loss with a KL term, forward and gradient in one pass.  With
+ * r = exp(logp - old_logp):
+ *   loss_partial[i] = w_i * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *                            + kl_coef * (exp(ref - logp) - (ref - logp) - 1))
+ *   dlogits = scaling * d loss / d logits,   *loss = sum_i loss_partial[i]
+ * weights NULL: w_i = 1 / rows.  A mean over the rows of a mask has w = mask /
+ * sum(mask).  ref_logp may be NULL if kl_coef is 0.  logp[i] is written too (0 for a
+ * row that does not count).  0 <= clip_low <= 1, clip_high >= 0. */
+int trb200_policy_loss_fused(const void* logits, int64_t logits_stride, const int32_t* actions, const float* old_logp,
+                             const float* ref_logp, const float* advantages, const float* weights,
+                             const float* scaling, float clip_low, float clip_high, float kl_coef, void* dlogits,
+                             int64_t dlogits_stride, float* logp, float* loss_partial, float* loss, int32_t rows,
+                             int32_t classes, int32_t dtype, void* stream);
+
+/* Paired preference loss (logistic loss of paired log ratios, with label smoothing),
+ * forward and gradient.  Sequence q owns the rows seq_starts[q] .. seq_starts[q+1] - 1
+ * (device, 2 * pairs + 1 ascending entries); sequences 2p and 2p + 1 are the preferred
+ * and the other answer of pair p.  With S_q = sum of logp over the rows of q that
+ * count (prompt rows carry a label outside [0, classes)) and
+ * x_p = beta * ((S_2p - S_2p+1) - (ref_2p - ref_2p+1)):
+ *   loss_partial[p] = (-(1 - label_smoothing) log sigmoid(x_p) - label_smoothing log sigmoid(-x_p)) / pairs
+ *   *loss = sum_p loss_partial[p],   dlogits = scaling * d loss / d logits
+ * ref_logp [2 * pairs] is the reference policy's S (NULL: 0).  logp [rows] and seq_logp
+ * [2 * pairs] are written too.  Rows in front of seq_starts[0] and behind
+ * seq_starts[2 * pairs] - 1 do not count.  Bounds outside [0, rows] are clamped; bounds
+ * that do not ascend give wrong sums but no access outside the buffers.
+ * workspace: trb200_preference_loss_workspace_bytes(rows), no contents expected. */
+size_t trb200_preference_loss_workspace_bytes(int32_t rows);
+int trb200_preference_loss_fused(const void* logits, int64_t logits_stride, const int32_t* labels,
+                                 const int32_t* seq_starts, const float* ref_logp, const float* scaling, double beta,
+                                 double label_smoothing, void* dlogits, int64_t dlogits_stride, float* logp,
+                                 float* seq_logp, float* loss_partial, float* loss, int32_t rows, int32_t pairs,
+                                 int32_t classes, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Classifier: fully connected layers of the AMP step.                        */
 /* FC_AMP_FWD / FC_AMP_BWD, src/backend/ops/dtensor/fc_op.cpp:259-480 (cuBLAS  */
 /* GEMMs + the bias kernels of fc_op.cu:20-101), with the ReLU                 */
@@ -513,6 +569,55 @@ int trb200_sgd_nesterov(float* weights, const float* grads, float* momentum, voi
  *   w = w*(1 - lr*wd) - lr*g/scaling */
 int trb200_sgd_plain(float* weights, const float* grads, void* weights_half, int64_t n, float lr,
                      float weight_decay, const float* scaling, const int32_t* skip_flag, void* stream);
+
+/* AdamW over many tensors in one launch, beside the SGD sweeps (which take one flat
+ * range): float master weights, gradients of one type, an optional 16-bit working copy,
+ * states in float or in 8 bits.
+ *   g = grad / scaling;  m = beta1*m + (1-beta1)*g;  v = beta2*v + (1-beta2)*g*g;  t = *step + 1
+ *   w = w*(1 - lr*weight_decay) - lr/(1-beta1^t) * m / (sqrt(v/(1-beta2^t)) + eps);  copy = 16 bit(w)
+ * 8-bit states are e4m3 codes (one byte an element) with a float scale per 128 elements
+ * of a tensor, value = code * scale, m rounded to nearest and v stochastically (random
+ * bits from Philox4x32-10 keyed by `seed`, counted by element, tensor and step); zeros
+ * in codes and scales are zero states.  A non-finite gradient in a step that is not
+ * skipped makes the 8-bit states of its 128 elements NaN.
+ *
+ * The plan: a description of the tensors that is written once on the host, copied to the
+ * device by the caller, and used by every step.  Tensors may be of any size and of any
+ * alignment of their elements; 16-byte aligned ones are faster.  No buffer that is
+ * written may overlap another one. */
+typedef struct trb200_adamw_tensor {
+    float* w;                  /* master weights, n floats                                  */
+    const void* g;             /* gradient, n elements of the plan's grad_dtype             */
+    void* m;                   /* first state, n floats or n e4m3 codes                     */
+    void* v;                   /* second state                                              */
+    float* m_scale;            /* 8-bit states: ceil(n / 128) floats each, else NULL        */
+    float* v_scale;
+    void* copy;                /* n elements of the plan's copy_dtype; ignored if that is NONE */
+    int64_t n;
+    float weight_decay;
+} trb200_adamw_tensor;
+
+typedef struct trb200_adamw_plan {
+    void* image;               /* device address of the copied image, 16-byte aligned: set by the caller */
+    int32_t count, chunks;     /* written by trb200_adamw_plan_write, as are the following  */
+    int32_t grad_dtype;        /* TRB200_DTYPE_F16, _BF16 or _F32                           */
+    int32_t copy_dtype;        /* TRB200_DTYPE_F16, _BF16 or _NONE                          */
+    int32_t state_bits;        /* 32 or 8                                                   */
+} trb200_adamw_plan;
+
+/* Bytes of the plan's image (0 for a bad description); `tensors` is a host array. */
+size_t trb200_adamw_plan_bytes(const trb200_adamw_tensor* tensors, int32_t count);
+/* Checks the tensors and writes the image to HOST memory, and *plan. */
+int trb200_adamw_plan_write(const trb200_adamw_tensor* tensors, int32_t count, int32_t grad_dtype, int32_t copy_dtype,
+                            int32_t state_bits, void* host_image, size_t image_bytes, trb200_adamw_plan* plan);
+/* One step.  `step` (device) counts the steps taken so far, >= 0, and is advanced by the
+ * kernel, so that a captured step can be replayed; lr_dev (device scalar, may be NULL)
+ * is used instead of lr.  Nothing at all happens if *skip_flag != 0 (the non-finite
+ * guard; NULL = never).  scaling: device scalar, NULL = 1.  Steps of one plan must not
+ * overlap one another.  0 <= beta < 1, eps > 0. */
+int trb200_adamw_step(const trb200_adamw_plan* plan, int32_t* step, float lr, const float* lr_dev, double beta1,
+                      double beta2, float eps, const float* scaling, const int32_t* skip_flag, uint64_t seed,
+                      void* stream);
 
 /* RANGE_CHECK_NAN with clipping (check_nan_and_clip_kernel, check_op.cu:54-79): a NaN
  * raises *flag and stays as it is (the optimizer then skips the step); every other

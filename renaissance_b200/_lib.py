@@ -50,6 +50,16 @@ class CbrBwdArgs(C.Structure):
     ]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("copy", C.c_void_p), ("n", C.c_int64), ("weight_decay", C.c_float)]
+
+
+class AdamWPlanDesc(C.Structure):
+    _fields_ = [("image", C.c_void_p), ("count", C.c_int32), ("chunks", C.c_int32), ("grad_dtype", C.c_int32),
+                ("copy_dtype", C.c_int32), ("state_bits", C.c_int32)]
+
+
 _lib = None
 
 
@@ -69,7 +79,7 @@ def load() -> C.CDLL:
             f"{LIB_PATH} is missing: build it with `python -m renaissance_b200.build` "
             "(there is no CPU or PyTorch fallback for these operators)")
     lib = C.CDLL(LIB_PATH)
-    vp, i32, i64, sz, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float
+    vp, i32, i64, sz, f32, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float, C.c_double
     pdesc = C.POINTER(ConvDesc)
     sig = {
         "trb200_last_error": (C.c_char_p, []),
@@ -109,6 +119,12 @@ def load() -> C.CDLL:
         "trb200_softmax_ce_bwd": (C.c_int, [vp, i64, vp, vp, vp, vp, vp, i64, i32, i32, vp]),
         "trb200_softmax_ce_fused": (C.c_int, [vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, vp]),
         "trb200_softmax_ce_fused_dtype": (C.c_int, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i32, i32, i32, vp]),
+        "trb200_token_logp": (C.c_int, [vp, i64, vp, vp, vp, i32, i32, i32, vp]),
+        "trb200_policy_loss_fused": (C.c_int, [vp, i64, vp, vp, vp, vp, vp, vp, f32, f32, f32, vp, i64, vp, vp, vp, i32,
+                                               i32, i32, vp]),
+        "trb200_preference_loss_workspace_bytes": (sz, [i32]),
+        "trb200_preference_loss_fused": (C.c_int, [vp, i64, vp, vp, vp, vp, f64, f64, vp, i64, vp, vp, vp, vp, i32, i32,
+                                                   i32, i32, vp, sz, vp]),
         "trb200_bn_stats_workspace_bytes": (sz, [i64, i32]),
         "trb200_bn_stats_finalize": (C.c_int, [vp, vp, vp, f32, f32, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32,
                                                vp, sz, vp]),
@@ -122,6 +138,10 @@ def load() -> C.CDLL:
         "trb200_sgd_momentum": (C.c_int, [vp, vp, vp, vp, i64, f32, f32, f32, vp, vp, vp]),
         "trb200_sgd_nesterov": (C.c_int, [vp, vp, vp, vp, i64, f32, f32, f32, vp, vp, vp]),
         "trb200_sgd_plain": (C.c_int, [vp, vp, vp, i64, f32, f32, vp, vp, vp]),
+        "trb200_adamw_plan_bytes": (sz, [C.POINTER(AdamWTensor), i32]),
+        "trb200_adamw_plan_write": (C.c_int, [C.POINTER(AdamWTensor), i32, i32, i32, i32, vp, sz,
+                                              C.POINTER(AdamWPlanDesc)]),
+        "trb200_adamw_step": (C.c_int, [C.POINTER(AdamWPlanDesc), vp, f32, vp, f64, f64, f32, vp, vp, C.c_uint64, vp]),
         "trb200_check_nan_and_clip": (C.c_int, [vp, i64, f32, vp, vp]),
         "trb200_grad_scaling": (C.c_int, [vp, vp, i32, vp]),
         "trb200_fc_amp_workspace_bytes": (sz, [i32, i32, i32]),

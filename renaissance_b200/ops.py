@@ -10,6 +10,8 @@ launcher derives them from its DTensors, and makes ONE C-ABI call.
     softmax_ce_amp_bwd     launch_softmax_ce_amp_bwd_cuda      softmax_ce_op.cpp:591-627
     softmax_ce_amp_fused   both nodes in one kernel
     mean_allreduce         launch_allreduce_cuda_impl          allreduce_op.cpp:37-105
+
+token_logprobs, policy_loss_fused, preference_loss_fused and AdamWPlan / adamw_step have no counterpart there.
 """
 from __future__ import annotations
 
@@ -610,6 +612,247 @@ def softmax_ce_amp_fused(logits, labels, scaling, label_smoothing, want_probs=Fa
                                       _ptr(dlogits), dlogits.stride(0), _ptr(part), _ptr(loss), _ptr(inv),
                                       b, k, _stream(stream)))
     return dict(loss=loss, inv_scaling=inv, probs=probs, loss_partial=part, dlogits=dlogits)
+
+
+# --------------------------------------------------------------------------- losses over chosen classes
+
+# storage types of logits and of AdamW's gradients
+FLOAT_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+class _On:
+    """Where a call runs: the tensors' device, and `stream` or that device's current one.  Allocations made inside
+    belong to that stream; tensors of another stream are held back from reuse until the call's work is done."""
+
+    def __init__(self, device, stream, tensors):
+        self.current = torch.cuda.current_stream(device)
+        self.stream = self.current if stream is None else stream
+        if self.stream.device != device:
+            raise ValueError(f"the stream belongs to {self.stream.device}, the tensors to {device}")
+        self.raw = self.stream.cuda_stream
+        self.device, self.tensors = device, tensors
+        self.contexts = []
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self.contexts.append(torch.cuda.device(self.device))
+        if self.raw != self.current.cuda_stream:
+            self.contexts.append(torch.cuda.stream(self.stream))
+        for c in self.contexts:
+            c.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        for c in reversed(self.contexts):
+            c.__exit__(*exc)
+        if self.raw != self.current.cuda_stream:
+            for t in self.tensors:
+                if t is not None:
+                    t.record_stream(self.stream)
+
+
+def _logit_rows(t, name):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2):
+        raise TypeError(f"{name}: 2-D CUDA tensor expected")
+    if t.dtype not in FLOAT_CODE:
+        raise TypeError(f"{name}: float16, bfloat16 or float32 expected, got {t.dtype}")
+    if t.shape[1] < 1 or max(t.shape) >= 1 << 31:
+        raise ValueError(f"{name}: 1 to 2^31 - 1 classes and fewer than 2^31 rows expected")
+    stride = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if (t.stride(1) != 1 and t.shape[1] > 1) or stride < t.shape[1]:
+        raise ValueError(f"{name}: unit column stride and rows that do not overlap expected (rows may be padded)")
+    return stride
+
+
+def _vector(t, n, dtype, name, device):
+    if not (isinstance(t, torch.Tensor) and t.device == device):
+        raise TypeError(f"{name}: tensor on {device} expected")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype {dtype} expected, got {t.dtype}")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: {n} consecutive elements expected, got shape {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _gradient_rows(dlogits, logits):
+    if dlogits is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+    stride = _logit_rows(dlogits, "dlogits")
+    if dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+        raise ValueError("dlogits: the logits' shape, type and device expected")
+    return dlogits, stride
+
+
+def token_logprobs(logits, labels, stream=None):
+    """Log-probability of each row's label and the row's log-sum-exp: dict(logp, lse), float [rows].  logits [rows,
+    classes] half, bfloat16 or float, labels int32.  A label outside [0, classes) gives 0 and 0 and its row is not
+    read; a row of minus infinities gives -inf and -inf."""
+    stride = _logit_rows(logits, "logits")
+    n, k = logits.shape
+    dev = logits.device
+    labels_p = _vector(labels, n, torch.int32, "labels", dev)
+    with _On(dev, stream, (logits, labels)) as on:
+        logp = torch.empty(n, dtype=torch.float32, device=dev)
+        lse = torch.empty(n, dtype=torch.float32, device=dev)
+        check(_lib.load().trb200_token_logp(logits.data_ptr(), stride, labels_p, logp.data_ptr(), lse.data_ptr(), n, k,
+                                            FLOAT_CODE[logits.dtype], on.raw))
+    return dict(logp=logp, lse=lse)
+
+
+def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0.2, clip_high=0.2, ref_logp=None,
+                      kl_coef=0.0, weights=None, dlogits=None, stream=None):
+    """Clipped policy loss, forward and gradient in one pass over the logits.  With r = exp(logp - old_logp):
+
+        loss = sum_i w_i * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(ref - logp) - (ref - logp) - 1))
+
+    logits [rows, classes] half, bfloat16 or float (rows may be padded), actions int32, the others float [rows];
+    weights default to 1 / rows (mask / mask.sum() for a mean over a mask).  Rows with weight 0 or an action outside
+    [0, classes) do not count: zero gradient, logits not read.  `scaling` (device scalar) multiplies dlogits only.
+    Returns dict(loss [1], loss_partial [rows], logp [rows], dlogits)."""
+    stride = _logit_rows(logits, "logits")
+    n, k = logits.shape
+    dev = logits.device
+    f32 = torch.float32
+    actions_p = _vector(actions, n, torch.int32, "actions", dev)
+    old_p = _vector(old_logp, n, f32, "old_logp", dev)
+    adv_p = _vector(advantages, n, f32, "advantages", dev)
+    scaling_p = _vector(scaling, 1, f32, "scaling", dev)
+    ref_p = None if ref_logp is None else _vector(ref_logp, n, f32, "ref_logp", dev)
+    weights_p = None if weights is None else _vector(weights, n, f32, "weights", dev)
+    with _On(dev, stream, (logits, actions, old_logp, advantages, scaling, ref_logp, weights, dlogits)) as on:
+        dlogits, dstride = _gradient_rows(dlogits, logits)
+        logp = torch.empty(n, dtype=f32, device=dev)
+        part = torch.empty(n, dtype=f32, device=dev)
+        loss = torch.empty(1, dtype=f32, device=dev)
+        check(_lib.load().trb200_policy_loss_fused(
+            logits.data_ptr(), stride, actions_p, old_p, ref_p, adv_p, weights_p, scaling_p, clip_low, clip_high, kl_coef,
+            dlogits.data_ptr(), dstride, logp.data_ptr(), part.data_ptr(), loss.data_ptr(), n, k,
+            FLOAT_CODE[logits.dtype], on.raw))
+    return dict(loss=loss, loss_partial=part, logp=logp, dlogits=dlogits)
+
+
+def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.1, label_smoothing=0.0, dlogits=None,
+                          stream=None):
+    """Paired preference loss (logistic loss of paired log ratios), forward and gradient.  Sequence q owns rows
+    seq_starts[q] .. seq_starts[q+1] - 1 of the logits (int32 [2 * pairs + 1], ascending, on the device); sequences 2p
+    and 2p + 1 are the preferred and the other answer of pair p, S_q the sum of logp over the rows of q whose label
+    lies in [0, classes).  With x_p = beta * ((S_2p - S_2p+1) - (ref_2p - ref_2p+1)):
+
+        loss = mean_p (-(1 - label_smoothing) * log sigmoid(x_p) - label_smoothing * log sigmoid(-x_p))
+
+    ref_logp [2 * pairs]: the reference policy's S (None: 0).  Rows outside every sequence do not count (zero
+    gradient).  Returns dict(loss [1], loss_partial [pairs], seq_logp [2 * pairs], logp [rows], dlogits)."""
+    stride = _logit_rows(logits, "logits")
+    n, k = logits.shape
+    dev = logits.device
+    f32 = torch.float32
+    labels_p = _vector(labels, n, torch.int32, "labels", dev)
+    if not isinstance(seq_starts, torch.Tensor) or seq_starts.numel() < 3 or seq_starts.numel() % 2 == 0:
+        raise ValueError("seq_starts: 2 * pairs + 1 entries of at least one pair expected")
+    seqs = seq_starts.numel() - 1
+    starts_p = _vector(seq_starts, seqs + 1, torch.int32, "seq_starts", dev)
+    ref_p = None if ref_logp is None else _vector(ref_logp, seqs, f32, "ref_logp", dev)
+    scaling_p = _vector(scaling, 1, f32, "scaling", dev)
+    lib = _lib.load()
+    with _On(dev, stream, (logits, labels, seq_starts, ref_logp, scaling, dlogits)) as on:
+        dlogits, dstride = _gradient_rows(dlogits, logits)
+        logp = torch.empty(n, dtype=f32, device=dev)
+        per_seq = torch.empty(seqs, dtype=f32, device=dev)
+        part = torch.empty(seqs // 2, dtype=f32, device=dev)
+        loss = torch.empty(1, dtype=f32, device=dev)
+        ws_bytes = lib.trb200_preference_loss_workspace_bytes(n)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        check(lib.trb200_preference_loss_fused(
+            logits.data_ptr(), stride, labels_p, starts_p, ref_p, scaling_p, beta, label_smoothing, dlogits.data_ptr(),
+            dstride, logp.data_ptr(), per_seq.data_ptr(), part.data_ptr(), loss.data_ptr(), n, seqs // 2, k,
+            FLOAT_CODE[logits.dtype], ws.data_ptr(), ws_bytes, on.raw))
+    return dict(loss=loss, loss_partial=part, seq_logp=per_seq, logp=logp, dlogits=dlogits)
+
+
+# --------------------------------------------------------------------------- AdamW over many tensors
+
+ADAMW_BLOCK = 128       # elements of a tensor that share one scale of an 8-bit state
+
+
+class AdamWPlan:
+    """The tensors that adamw_step updates, checked and laid out once.  All are lists with one CUDA tensor per
+    parameter, contiguous, of any size: `weights` float, `grads` of one type (half, bfloat16 or float), states `m` and
+    `v` either float or torch.float8_e4m3fn; the latter with `m_scales` and `v_scales`, float [ceil(n / 128)] each
+    (value = code * scale; zeros to start with).  `copies`: 16-bit working copies that every step refreshes, or None.
+    `weight_decay`: one number or one per tensor.  The plan keeps the tensors: a gradient has to stay in the buffer
+    that it was given with."""
+
+    def __init__(self, weights, grads, m, v, m_scales=None, v_scales=None, copies=None, weight_decay=0.0):
+        weights = list(weights)
+        count = len(weights)
+        decay = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else [float(x) for x in weight_decay]
+        lists = {"weights": weights, "grads": list(grads), "m": list(m), "v": list(v)}
+        eight = len(lists["m"]) > 0 and lists["m"][0].dtype == torch.float8_e4m3fn
+        if (m_scales is not None) != eight or (v_scales is not None) != eight:
+            raise ValueError("AdamWPlan: 8-bit states need m_scales and v_scales, float states have none")
+        if eight:
+            lists["m_scales"], lists["v_scales"] = list(m_scales), list(v_scales)
+        if copies is not None:
+            lists["copies"] = list(copies)
+        for name, ts in lists.items():
+            if len(ts) != count:
+                raise ValueError(f"AdamWPlan: {name} has {len(ts)} tensors, weights {count}")
+        if len(decay) != count:
+            raise ValueError(f"AdamWPlan: weight_decay has {len(decay)} entries, weights {count}")
+        if count == 0:
+            raise ValueError("AdamWPlan: no tensors")
+        self.device = weights[0].device
+        if self.device.type != "cuda":
+            raise TypeError("AdamWPlan: CUDA tensors expected")
+        state = torch.float8_e4m3fn if eight else torch.float32
+        grad = lists["grads"][0].dtype
+        if grad not in FLOAT_CODE:
+            raise TypeError(f"AdamWPlan: gradients of type {grad}")
+        copy = lists["copies"][0].dtype if copies is not None else None
+        if copy is not None and copy not in DTYPE_CODE:
+            raise TypeError(f"AdamWPlan: float16 or bfloat16 copies expected, got {copy}")
+        kinds = {"weights": torch.float32, "grads": grad, "m": state, "v": state, "m_scales": torch.float32,
+                 "v_scales": torch.float32, "copies": copy}
+        table = (_lib.AdamWTensor * count)()
+        fields = {"weights": "w", "grads": "g", "m": "m", "v": "v", "m_scales": "m_scale", "v_scales": "v_scale", "copies": "copy"}
+        for i, w in enumerate(weights):
+            n = w.numel()
+            for name, ts in lists.items():
+                want = -(-n // ADAMW_BLOCK) if name.endswith("scales") else n
+                setattr(table[i], fields[name], _vector(ts[i], want, kinds[name], f"{name}[{i}]", self.device))
+            table[i].n, table[i].weight_decay = n, decay[i]
+        lib = _lib.load()
+        host = torch.zeros(max(1, lib.trb200_adamw_plan_bytes(table, count)), dtype=torch.uint8)
+        self.desc = _lib.AdamWPlanDesc()
+        check(lib.trb200_adamw_plan_write(table, count, FLOAT_CODE[grad], -1 if copy is None else DTYPE_CODE[copy],
+                                          8 if eight else 32, host.data_ptr(), host.numel(), C.byref(self.desc)))
+        self.image = host.to(self.device)
+        self.desc.image = self.image.data_ptr()
+        self.tensors = lists
+
+
+def adamw_step(plan, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, scaling=None, skip_flag=None, seed=0, stream=None):
+    """One AdamW step over the plan's tensors, in one launch (decoupled weight decay, bias correction):
+
+        g = grad / scaling;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  t = step + 1
+        w = w (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps);  copy = 16-bit w
+
+    `step`: int32 device scalar, the steps taken so far; the kernel advances it, so a captured step can be replayed.
+    `lr`: a number, or a float device scalar that a schedule writes between replays.  Nothing happens where the device
+    scalar `skip_flag` (int32) is not 0.  `seed` keys the stochastic rounding of 8-bit second moments."""
+    if not isinstance(plan, AdamWPlan):
+        raise TypeError("adamw_step: an AdamWPlan expected")
+    dev = plan.device
+    step_p = _vector(step, 1, torch.int32, "step", dev)
+    lr_p, lr_v = (_vector(lr, 1, torch.float32, "lr", dev), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
+    scaling_p = None if scaling is None else _vector(scaling, 1, torch.float32, "scaling", dev)
+    skip_p = None if skip_flag is None else _vector(skip_flag, 1, torch.int32, "skip_flag", dev)
+    held = (step, lr if lr_p else None, scaling, skip_flag)
+    if stream is not None:
+        held += (plan.image, *(t for ts in plan.tensors.values() for t in ts))
+    with _On(dev, stream, held) as on:
+        check(_lib.load().trb200_adamw_step(C.byref(plan.desc), step_p, lr_v, lr_p, beta1, beta2, eps, scaling_p, skip_p,
+                                            seed, on.raw))
 
 
 # --------------------------------------------------------------------------- classifier

@@ -207,6 +207,11 @@ __device__ __forceinline__ uint32_t code_stochastic(float y, uint32_t r) {
 // largest of non-negative floats over the warp, NaN above all (bits of such floats order as integers)
 __device__ __forceinline__ float warp_top(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 
+// an infinite largest value leaves nothing to scale by: NaN, as for a NaN
+__device__ __forceinline__ float scale_of(float top) {
+    return top < kSmallest ? 0.f : (top == INFINITY ? NAN : __fmul_rn(top, 1.0f / kE4m3Max));
+}
+
 // One scale block by one warp: lane l has elements 4l .. 4l + 3; `r` = their random halves.
 template <int GT, int CT>
 __device__ __forceinline__ void block_8bit(const Tensor& t, int64_t block, int64_t n, const uint32_t (&r)[4], const Hyper& h,
@@ -269,8 +274,8 @@ __device__ __forceinline__ void block_8bit(const Tensor& t, int64_t block, int64
             }
     }
     if (lane == 0) {
-        t.m_scale[block] = mt < kSmallest ? 0.f : __fmul_rn(mt, 1.0f / kE4m3Max);
-        t.v_scale[block] = vt < kSmallest ? 0.f : __fmul_rn(vt, 1.0f / kE4m3Max);
+        t.m_scale[block] = scale_of(mt);
+        t.v_scale[block] = scale_of(vt);
     }
 }
 

@@ -384,8 +384,9 @@ def test_results_are_reproducible_and_other_streams_agree():
         torch.cuda.synchronize()
         for k in ("loss", "loss_partial", "logp"):
             assert torch.equal(a[k], first[k]) and torch.equal(c[k], first[k])
-        assert torch.equal(a["dlogits"], first["dlogits"]) and torch.equal(b["dlogits"], pref["dlogits"])
-        assert torch.equal(b["loss"], pref["loss"])
+        bits = lambda t: t.view(torch.int16)        # one row is NaN in the preference loss, which does not mask it
+        assert torch.equal(bits(a["dlogits"]), bits(first["dlogits"])) and torch.equal(bits(b["dlogits"]), bits(pref["dlogits"]))
+        assert torch.equal(bits(b["loss"]), bits(pref["loss"]))
 
 
 def test_captured_calls_replay_beside_eager_ones():

@@ -599,7 +599,7 @@ typedef struct trb200_adamw_tensor {
 
 typedef struct trb200_adamw_plan {
     void* image;               /* device address of the copied image, 16-byte aligned: set by the caller */
-    int32_t count, chunks;     /* written by trb200_adamw_plan_write, as are the following  */
+    int32_t count, units;      /* written by trb200_adamw_plan_write, as are the following  */
     int32_t grad_dtype;        /* TRB200_DTYPE_F16, _BF16 or _F32                           */
     int32_t copy_dtype;        /* TRB200_DTYPE_F16, _BF16 or _NONE                          */
     int32_t state_bits;        /* 32 or 8                                                   */

@@ -56,7 +56,7 @@ class AdamWTensor(C.Structure):
 
 
 class AdamWPlanDesc(C.Structure):
-    _fields_ = [("image", C.c_void_p), ("count", C.c_int32), ("chunks", C.c_int32), ("grad_dtype", C.c_int32),
+    _fields_ = [("image", C.c_void_p), ("count", C.c_int32), ("units", C.c_int32), ("grad_dtype", C.c_int32),
                 ("copy_dtype", C.c_int32), ("state_bits", C.c_int32)]
 
 

@@ -330,6 +330,10 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// its two halves, for work in between; a CTA that has passed the wait knows that its peers run
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // One arrival on a barrier of another CTA of the cluster.  No cluster-scope release: what the waiter depends on
 // (tensor-memory reads) is ordered by tcgen05.fence + a block barrier before this, and a cluster-scope release
 // issued by a thread with a bulk store in flight was measured to stall that thread for ~1800 clocks.

@@ -17,14 +17,20 @@
 // logits are not read.
 //
 // All of it is bound by HBM: per logit one read, and one write where there is a gradient.
+#include "chained.cuh"
 #include "common.cuh"
+#include "packed.cuh"
+#include "sm100_ptx.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace trb {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+// log2(e) in two floats: with the first alone every exponent is 1.3e-8 of itself short, and log s, whose terms are all
+// off the same way, by 1.3e-7 at 100 000 classes (measured), which a sequence of 1000 rows adds up
+constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596303e-8f;
 
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -100,28 +106,30 @@ __device__ __forceinline__ void store_any(void* p, const uint4& v, int elem) {
 }
 
 // ---------------------------------------------------------------- maximum and sum of exponentials
-// s counts exponentials against m.  m = -inf goes with s = 0 (nothing but -inf seen); a NaN ends up in s.
-struct MaxSum { float m, s; };
+// exp(z - m) is 2^(d hi + d lo) with d = z - m: the difference first, so that the largest element gives exactly 1, a row
+// with one class exactly logp = 0, and the type's lowest value as a mask no overflow.
+struct MaxSum { float m, s; };       // s: sum of exp(z - m); m = -inf goes with s = 0; a NaN ends up in s
 
-// the number exponentials are taken against: 0 stands in for -inf, so that no difference of infinities is formed
+__device__ __forceinline__ float exp_of(float d) { return fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi)); }
+
+// what differences are taken to: 0 stands in for -inf, so that no difference of infinities is formed
 __device__ __forceinline__ float pivot(float m) { return m == -INFINITY ? 0.f : m; }
 
 __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b) {
     const float m = fmaxf(a.m, b.m), p = pivot(m);
-    return {m, a.s * fast_exp2((a.m - p) * kLog2e) + b.s * fast_exp2((b.m - p) * kLog2e)};
+    return {m, a.s * exp_of(a.m - p) + b.s * exp_of(b.m - p)};
 }
 
 template <int N>
 __device__ __forceinline__ void take(MaxSum& a, const float (&f)[N]) {
-    float m = a.m;
+    float m = f[0];
 #pragma unroll
-    for (int j = 0; j < N; ++j) m = fmaxf(m, f[j]);
+    for (int j = 1; j < N; ++j) m = fmaxf(m, f[j]);
+    m = fmaxf(m, a.m);
     const float p = pivot(m);
-    float s = a.s * fast_exp2((a.m - p) * kLog2e);
-    // the difference is taken before the scaling: with the type's lowest value as mask, z * log2(e) would overflow
+    a = {m, a.s * exp_of(a.m - p)};
 #pragma unroll
-    for (int j = 0; j < N; ++j) s += fast_exp2((f[j] - p) * kLog2e);
-    a = {m, s};
+    for (int j = 0; j < N; ++j) a.s += exp_of(f[j] - p);
 }
 
 // the same MaxSum in every thread of a block of T threads; s_red holds T / 32 entries
@@ -131,13 +139,151 @@ __device__ __forceinline__ MaxSum block_merge(MaxSum a, MaxSum* s_red) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         a = merge(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+    __syncthreads();
     if (lane == 0) s_red[warp] = a;
     __syncthreads();
-    a = lane < T / 32 ? s_red[lane] : MaxSum{-INFINITY, 0.f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        a = merge(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+    a = s_red[0];
+#pragma unroll 1
+    for (int i = 1; i < T / 32; ++i) a = merge(a, s_red[i]);
     return a;
+}
+
+// ---- rows whose maximum lies within +-kPlain; others leave for the code above
+constexpr float kPlain = 256.f;
+constexpr float kFloor = -1.26765060e30f;   // -2^100: stands in for -inf as a thread's maximum
+
+__device__ __forceinline__ bool plain(float m) { return fabsf(m) <= kPlain; }
+
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+    const float2 f = split(x);
+    return pair_of(fast_exp2(f.x), fast_exp2(f.y));
+}
+// exp_of() of z - m; `minus` = -m twice
+__device__ __forceinline__ uint64_t exp_pair(uint64_t z, uint64_t minus) {
+    const uint64_t d = add2(z, minus);
+    return exp2_pair(fma2(d, twice(kLog2eLo), mul2(d, twice(kLog2eHi))));
+}
+
+// MaxSum over the low N lanes of a warp (N a power of two); the maximum first, so that a lane rescales its sum once
+template <int N>
+__device__ __forceinline__ MaxSum warp_merge(MaxSum a) {
+    float m = a.m;
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = a.s * exp_of(a.m - m);
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return {m, s};
+}
+
+// Vectors of a row as pairs of floats.
+template <int DT>
+struct Vec {
+    using L = Logit<DT>;
+    static constexpr int kPairs = L::kVec / 2;
+    // -inf in every element
+    static constexpr uint32_t kLow = DT == TRB200_DTYPE_F16 ? 0xfc00fc00u : (DT == TRB200_DTYPE_BF16 ? 0xff80ff80u : 0xff800000u);
+
+    static __device__ __forceinline__ uint64_t pair(const uint4& v, int i) {
+        if constexpr (DT == TRB200_DTYPE_F32) {
+            return i == 0 ? pair_of(__uint_as_float(v.x), __uint_as_float(v.y)) : pair_of(__uint_as_float(v.z), __uint_as_float(v.w));
+        } else {
+            const float2 f = unpack2_t<L::kBf16>(i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)));
+            return pair_of(f.x, f.y);
+        }
+    }
+
+    // largest element of N vectors, NaN aside; 16-bit types two at a time
+    template <int N>
+    static __device__ __forceinline__ float top(const uint4 (&v)[N]) {
+        if constexpr (DT == TRB200_DTYPE_F32) {
+            float m = __uint_as_float(v[0].x);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y))),
+                          fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w)));
+            return m;
+        } else {
+            using H = std::conditional_t<L::kBf16, __nv_bfloat162, __half2>;
+            const H* h = reinterpret_cast<const H*>(&v);
+            H m[4] = {h[0], h[1], h[2], h[3]};          // four chains
+#pragma unroll
+            for (int i = 4; i < 4 * N; ++i) m[i & 3] = __hmax2(m[i & 3], h[i]);
+            m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+            return fmaxf(__low2float(m[0]), __high2float(m[0]));
+        }
+    }
+};
+
+// Maximum and sum over vectors that arrive in groups of N.
+struct Running {
+    float m = kFloor;
+    uint64_t s0 = 0, s1 = 0;            // two sums of pairs, to shorten the chains of additions
+
+    __device__ __forceinline__ uint64_t raise(float top) {
+        const uint64_t sc = twice(exp_of(m - top));
+        m = top;
+        s0 = mul2(s0, sc);
+        s1 = mul2(s1, sc);
+        return twice(-top);
+    }
+
+    template <int DT, int N>
+    __device__ __forceinline__ void take(const uint4 (&v)[N]) {
+        using V = Vec<DT>;
+        const uint64_t minus = raise(fmaxf(m, V::top(v)));
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+#pragma unroll
+            for (int i = 0; i < V::kPairs; i += 2) {
+                s0 = add2(s0, exp_pair(V::pair(v[k], i), minus));
+                s1 = add2(s1, exp_pair(V::pair(v[k], i + 1), minus));
+            }
+        }
+    }
+
+    // one element, -inf for none
+    __device__ __forceinline__ void take_one(float z) {
+        raise(fmaxf(m, z));
+        s0 = add2(s0, pair_of(exp_of(z - m), 0.f));
+    }
+
+    __device__ __forceinline__ MaxSum total() const {
+        const float2 s = split(add2(s0, s1));
+        return {m, s.x + s.y};
+    }
+};
+
+// What the gradient of a row needs: g_c = coef ([c == y] - exp(z_c - m) / s).  A 16-bit result is one multiply-add and
+// one exponential, |coef| p_c = 2^(z_c hi + up) with up = log2(|coef| / s) - m hi (within kPlain its rounding is 2^-15
+// of a power, next to the 2^-9 of the result's), and the sign is the conversion's.
+struct Slope {
+    float m, s, coef, up;
+    __device__ __forceinline__ float at(float z, bool label) const {        // one element in full precision
+        return fmaf(exp_of(z - m), -coef / s, label ? coef : 0.f);
+    }
+};
+
+__device__ __forceinline__ Slope slope_of(MaxSum a, float coef) {
+    return {a.m, a.s, coef, log2f(fabsf(coef) / a.s) - a.m * kLog2eHi};
+}
+
+template <int DT, bool NEG>
+__device__ __forceinline__ uint4 slope_vec(const uint4& v, const Slope& g) {
+    using V = Vec<DT>;
+    if constexpr (DT == TRB200_DTYPE_F32) {
+        const uint64_t minus = twice(-g.m), fall = twice(-g.coef / g.s);
+        const float2 x = split(mul2(exp_pair(V::pair(v, 0), minus), fall)), y = split(mul2(exp_pair(V::pair(v, 1), minus), fall));
+        return make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
+    } else {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 x = split(exp2_pair(fma2(V::pair(v, i), twice(kLog2eHi), twice(g.up))));
+            o[i] = NEG ? pack2_t<V::L::kBf16>(-x.x, -x.y) : pack2_t<V::L::kBf16>(x.x, x.y);
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
 }
 
 // ---------------------------------------------------------------- what a row's loss is
@@ -151,36 +297,119 @@ struct PolicyArgs {
     float even_weight;          // 1 / rows
 };
 
-// weighted loss of a row and its derivative with respect to logp
-__device__ __forceinline__ void policy_row(const PolicyArgs& a, int row, float w, float logp, float& loss, float& slope) {
-    const float adv = a.advantages[row];
-    const float ratio = expf(logp - a.old_logp[row]);
+struct PolicyIn { float old_logp, ref_logp, advantage, weight, scaling; };
+
+__device__ __forceinline__ PolicyIn policy_in(const PolicyArgs& a, int row) {
+    return {a.old_logp[row], a.ref_logp ? a.ref_logp[row] : 0.f, a.advantages[row],
+            a.weights ? a.weights[row] : a.even_weight, a.scaling[0]};
+}
+
+// weighted loss of a row and scaling * its derivative with respect to logp
+__device__ __forceinline__ void policy_row(const PolicyArgs& a, const PolicyIn& in, float logp, float& loss, float& coef) {
+    const float adv = in.advantage;
+    const float ratio = expf(logp - in.old_logp);
     const float kept = ratio * adv;
     const float cut = fminf(fmaxf(ratio, a.low), a.high) * adv;
     float l, g;
     if (kept <= cut) { l = -kept; g = -kept; }
     else { l = kept > cut ? -cut : NAN; g = kept > cut ? 0.f : NAN; }     // unordered: a NaN stays one
     if (a.ref_logp) {
-        const float gap = a.ref_logp[row] - logp;
+        const float gap = in.ref_logp - logp;
         const float more = expm1f(gap);                         // no cancellation next to gap = 0
         l += a.kl_coef * (more - gap);
         g -= a.kl_coef * more;
     }
-    loss = l * w;
-    slope = g * w;
+    loss = l * in.weight;
+    coef = g * in.weight * in.scaling;
 }
 
-// ---------------------------------------------------------------- row kernels
+// ---------------------------------------------------------------- what a row kernel is for
 template <int DT>
 struct Rows {
-    const typename Logit<DT>::T* z;
+    using T = typename Logit<DT>::T;
+    const T* z;
     int64_t z_stride;
-    typename Logit<DT>::T* d;       // gradient
+    T* d;                           // gradient
     int64_t d_stride;
     const int32_t* labels;
-    int classes;
+    int rows, classes;
+    __device__ __forceinline__ const T* logits(int row) const { return z + (int64_t)row * z_stride; }
+    __device__ __forceinline__ T* gradient(int row) const { return d + (int64_t)row * d_stride; }
 };
 
+// log-probability of the label with logit zy; never above 0
+__device__ __forceinline__ float label_logp(float zy, MaxSum a) { return (zy - a.m) - logf(a.s); }
+
+// Each purpose says which rows count, takes a counting row's MaxSum to its outputs and, for a gradient, to coef.
+struct LogpRows {
+    static constexpr bool kGradient = false;
+    float* logp;
+    float* lse;
+    struct In {};
+    __device__ __forceinline__ bool counts(int row) const { return true; }
+    __device__ __forceinline__ In in(int row) const { return {}; }
+    __device__ __forceinline__ void skip(int row) const {
+        logp[row] = 0.f;
+        if (lse) lse[row] = 0.f;
+    }
+    __device__ __forceinline__ float finish(int row, const In&, float zy, MaxSum a, bool write) const {
+        if (write) {
+            const bool none = a.s == 0.f;                           // every logit is -inf
+            logp[row] = none ? -INFINITY : label_logp(zy, a);
+            if (lse) lse[row] = none ? -INFINITY : a.m + logf(a.s);
+        }
+        return 0.f;
+    }
+};
+
+struct PolicyRows {
+    static constexpr bool kGradient = true;
+    PolicyArgs p;
+    float* logp;
+    float* loss_partial;
+    using In = PolicyIn;
+    __device__ __forceinline__ bool counts(int row) const { return !p.weights || p.weights[row] != 0.f; }
+    __device__ __forceinline__ In in(int row) const { return policy_in(p, row); }
+    __device__ __forceinline__ void skip(int row) const { logp[row] = loss_partial[row] = 0.f; }
+    __device__ __forceinline__ float finish(int row, const In& x, float zy, MaxSum a, bool write) const {
+        float lp = 0.f, loss = 0.f, coef = 0.f;
+        if (a.s != 0.f) {
+            lp = label_logp(zy, a);
+            policy_row(p, x, lp, loss, coef);
+        }
+        if (write) {
+            logp[row] = lp;
+            loss_partial[row] = loss;
+        }
+        return coef;
+    }
+};
+
+// first pass of the preference loss: statistics of the rows that count; coef starts at 0 for every row
+struct PairRows {
+    static constexpr bool kGradient = false;
+    const int32_t* seq_starts;
+    int seqs;
+    float* logp;
+    float* row_max;
+    float* row_sum;                 // 0: the row does not count
+    float* coef;
+    struct In {};
+    __device__ __forceinline__ bool counts(int row) const { return row >= seq_starts[0] && row < seq_starts[seqs]; }
+    __device__ __forceinline__ In in(int row) const { return {}; }
+    __device__ __forceinline__ void skip(int row) const { logp[row] = row_max[row] = row_sum[row] = coef[row] = 0.f; }
+    __device__ __forceinline__ float finish(int row, const In&, float zy, MaxSum a, bool write) const {
+        if (write) {
+            logp[row] = a.s != 0.f ? label_logp(zy, a) : 0.f;
+            row_max[row] = a.m;
+            row_sum[row] = a.s;
+            coef[row] = 0.f;
+        }
+        return 0.f;
+    }
+};
+
+// ---------------------------------------------------------------- rows that leave the plain path
 // maximum and sum of the row over the T threads of the block
 template <int DT, int T>
 __device__ __forceinline__ MaxSum row_stats(const typename Logit<DT>::T* z, int classes, MaxSum* s_red) {
@@ -188,23 +417,13 @@ __device__ __forceinline__ MaxSum row_stats(const typename Logit<DT>::T* z, int 
     const RowSplit sp(z, classes);
     MaxSum a{-INFINITY, 0.f};
     const int e = sp.single(threadIdx.x, classes);
-    if (e >= 0) a = {L::load(z + e), 1.0f};
-    if (a.m == -INFINITY) a.s = 0.f;
-    if (isnan(a.m)) a = {-INFINITY, NAN};
-    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
-    int v = threadIdx.x;
-    for (; v + 3 * T < sp.nvec; v += 4 * T) {           // four loads in flight
-        uint4 raw[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) raw[u] = zv[v + u * T];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float f[L::kVec];
-            L::unpack(raw[u], f);
-            take(a, f);
-        }
+    if (e >= 0) {
+        const float f[1] = {L::load(z + e)};
+        take(a, f);
     }
-    for (; v < sp.nvec; v += T) {
+    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
+#pragma unroll 1
+    for (int v = threadIdx.x; v < sp.nvec; v += T) {
         float f[L::kVec];
         L::unpack(zv[v], f);
         take(a, f);
@@ -212,118 +431,258 @@ __device__ __forceinline__ MaxSum row_stats(const typename Logit<DT>::T* z, int 
     return block_merge<T>(a, s_red);
 }
 
-// d = coef * ([c == y] - exp(z - m) / s) over the T threads of the block; coef == 0 writes zeros without reading z
+// zeros for the vectors [first, last) of a row and, for the block that is told so, its single elements
+template <int DT, int T>
+__device__ __forceinline__ void zero_row(typename Logit<DT>::T* d, int classes, int tid, int part, int parts) {
+    const RowSplit sp(d, classes);
+    const int e = part == 0 ? sp.single(tid, classes) : -1;
+    if (e >= 0) Logit<DT>::store(d + e, 0.f);
+    uint4* dv = reinterpret_cast<uint4*>(d + sp.head);
+#pragma unroll 4
+    for (int v = part * T + tid; v < sp.nvec; v += parts * T) __stcs(dv + v, make_uint4(0u, 0u, 0u, 0u));
+}
+
+// d = coef * ([c == y] - exp(z - m) / s) over the T threads of the block
 template <int DT, int T>
 __device__ __forceinline__ void row_gradient(const typename Logit<DT>::T* z, typename Logit<DT>::T* d, int classes,
-                                             int y, float m, float s, float coef) {
+                                             int y, MaxSum a, float coef) {
     using L = Logit<DT>;
-    constexpr int kSize = (int)sizeof(typename L::T);
-    if (coef == 0.f) {
-        const RowSplit sp(d, classes);
-        const int e = sp.single(threadIdx.x, classes);
-        if (e >= 0) L::store(d + e, 0.f);
-        uint4* dv = reinterpret_cast<uint4*>(d + sp.head);
-        for (int v = threadIdx.x; v < sp.nvec; v += T) dv[v] = make_uint4(0u, 0u, 0u, 0u);
-        return;
-    }
     const RowSplit sp(z, classes);
-    const float p = pivot(m), fall = -coef / s;
+    const float p = pivot(a.m), fall = -coef / a.s;
     const int e = sp.single(threadIdx.x, classes);
-    if (e >= 0) L::store(d + e, fmaf(fast_exp2((L::load(z + e) - p) * kLog2e), fall, e == y ? coef : 0.f));
+    if (e >= 0) L::store(d + e, fmaf(exp_of(L::load(z + e) - p), fall, e == y ? coef : 0.f));
     const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
-    auto one = [&](const uint4& raw, int v) {
+#pragma unroll 1
+    for (int v = threadIdx.x; v < sp.nvec; v += T) {
         float f[L::kVec];
-        L::unpack(raw, f);
-#pragma unroll
-        for (int j = 0; j < L::kVec; ++j) f[j] = fast_exp2((f[j] - p) * kLog2e) * fall;
+        L::unpack(zv[v], f);
         const int c0 = sp.head + v * L::kVec, jy = y - c0;
-        if ((unsigned)jy < (unsigned)L::kVec) {                 // the label sits in at most one vector of the row
 #pragma unroll
-            for (int j = 0; j < L::kVec; ++j) f[j] += j == jy ? coef : 0.f;
-        }
-        store_any(d + c0, L::pack(f), kSize);
-    };
-    int v = threadIdx.x;
-    for (; v + 3 * T < sp.nvec; v += 4 * T) {
-        uint4 raw[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) raw[u] = zv[v + u * T];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) one(raw[u], v + u * T);
+        for (int j = 0; j < L::kVec; ++j) f[j] = fmaf(exp_of(f[j] - p), fall, j == jy ? coef : 0.f);
+        store_any(d + c0, L::pack(f), (int)sizeof(typename L::T));
     }
-    for (; v < sp.nvec; v += T) one(zv[v], v);
 }
 
-// log-probability of the label; a row that is read has 0 <= y < classes
-template <int DT>
-__device__ __forceinline__ float label_logp(const typename Logit<DT>::T* z, int y, MaxSum a) {
-    return (Logit<DT>::load(z + y) - pivot(a.m)) - logf(a.s);
+// ---------------------------------------------------------------- short rows: one warp each, in registers
+constexpr int kShortWarps = 4;
+
+template <int DT, int K>
+__device__ __forceinline__ void store_slopes(const uint4 (&raw)[K], typename Logit<DT>::T* dv, int v0, int nvec, const Slope& g) {
+    constexpr int kVec = Logit<DT>::kVec;
+    const bool wide = (reinterpret_cast<uintptr_t>(dv) & 15u) == 0, neg = g.coef > 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int v = v0 + 32 * k;
+        if (v >= nvec) continue;
+        const uint4 out = neg ? slope_vec<DT, true>(raw[k], g) : slope_vec<DT, false>(raw[k], g);
+        if (wide) __stcs(reinterpret_cast<uint4*>(dv) + v, out);
+        else store_any(dv + (int64_t)v * kVec, out, (int)sizeof(typename Logit<DT>::T));
+    }
 }
 
-template <int DT, int T>
-__global__ void __launch_bounds__(T)
-token_logp_rows(Rows<DT> r, float* __restrict__ logp, float* __restrict__ lse) {
-    __shared__ MaxSum s_red[T / 32];
-    const int row = blockIdx.x;
+template <int DT, int K, class P>
+__global__ void __launch_bounds__(32 * kShortWarps)
+rows_short(Rows<DT> r, P p) {
+    using L = Logit<DT>;
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x * kShortWarps + (threadIdx.x >> 5);
+    ptx::wait_prior_grid();
+    ptx::let_next_grid_start();
+    if (row >= r.rows) return;
     const int y = r.labels[row];
-    if ((unsigned)y >= (unsigned)r.classes) {
-        if (threadIdx.x == 0) {
-            logp[row] = 0.f;
-            if (lse) lse[row] = 0.f;
-        }
+    const auto* z = r.logits(row);
+    if ((unsigned)y >= (unsigned)r.classes || !p.counts(row)) {
+        if (lane == 0) p.skip(row);
+        if constexpr (P::kGradient) zero_row<DT, 32>(r.gradient(row), r.classes, lane, 0, 1);
         return;
     }
-    const auto* z = r.z + (int64_t)row * r.z_stride;
-    const MaxSum a = row_stats<DT, T>(z, r.classes, s_red);
-    if (threadIdx.x == 0) {
-        const bool none = a.s == 0.f;                           // every logit is -inf
-        logp[row] = none ? -INFINITY : label_logp<DT>(z, y, a);
-        if (lse) lse[row] = none ? -INFINITY : a.m + logf(a.s);
+    const RowSplit sp(z, r.classes);
+    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
+    uint4 raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        raw[k] = make_uint4(Vec<DT>::kLow, Vec<DT>::kLow, Vec<DT>::kLow, Vec<DT>::kLow);
+        if (lane + 32 * k < sp.nvec) raw[k] = __ldcs(zv + lane + 32 * k);
     }
-}
-
-template <int DT, int T>
-__global__ void __launch_bounds__(T)
-policy_loss_rows(Rows<DT> r, PolicyArgs p, float* __restrict__ logp, float* __restrict__ loss_partial) {
-    __shared__ MaxSum s_red[T / 32];
-    const int row = blockIdx.x;
-    const int y = r.labels[row];
-    const float w = p.weights ? p.weights[row] : p.even_weight;
-    const auto* z = r.z + (int64_t)row * r.z_stride;
-    float lp = 0.f, loss = 0.f, coef = 0.f;
-    MaxSum a{0.f, 1.f};
-    if ((unsigned)y < (unsigned)r.classes && w != 0.f) {
-        a = row_stats<DT, T>(z, r.classes, s_red);
-        if (a.s != 0.f) {
-            lp = label_logp<DT>(z, y, a);
-            policy_row(p, row, w, lp, loss, coef);
-            coef *= p.scaling[0];
+    const int edge_at = sp.single(lane, r.classes);
+    const float edge = edge_at >= 0 ? L::load(z + edge_at) : -INFINITY;
+    const auto in = p.in(row);
+    const float zy = L::load(z + y);
+    Running run;
+    run.template take<DT>(raw);
+    run.take_one(edge);
+    MaxSum a = warp_merge<32>(run.total());
+    if (!plain(a.m)) {                                          // seldom
+        a = {-INFINITY, 0.f};
+        if (edge_at >= 0) {
+            float f[1] = {edge};
+            take(a, f);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float f[L::kVec];
+            L::unpack(raw[k], f);
+            take(a, f);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            a = merge(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+    }
+    const float coef = p.finish(row, in, zy, a, lane == 0);     // the same in all lanes
+    if constexpr (P::kGradient) {
+        auto* d = r.gradient(row);
+        if (coef == 0.f) {
+            zero_row<DT, 32>(d, r.classes, lane, 0, 1);
+        } else if (plain(a.m)) {
+            const Slope g = slope_of(a, coef);
+            auto* dv = d + sp.head;
+            store_slopes<DT, K>(raw, dv, lane, sp.nvec, g);
+            if (edge_at >= 0) L::store(d + edge_at, g.at(edge, edge_at == y));
+            // the label's element again, by the lane that stored its vector
+            const int vy = (y - sp.head) / L::kVec;
+            if (y >= sp.head && vy < sp.nvec && (vy & 31) == lane) L::store(d + y, g.at(zy, true));
+        } else {
+            const float m = pivot(a.m), fall = -coef / a.s;
+            for (int c = lane; c < r.classes; c += 32)
+                L::store(d + c, fmaf(exp_of(L::load(z + c) - m), fall, c == y ? coef : 0.f));
         }
     }
-    if (threadIdx.x == 0) {
-        logp[row] = lp;
-        loss_partial[row] = loss;
-    }
-    row_gradient<DT, T>(z, r.d + (int64_t)row * r.d_stride, r.classes, y, a.m, a.s, coef);
 }
 
-// first pass of the preference loss: statistics of the rows that count; coef starts at 0 for every row
-template <int DT, int T>
-__global__ void __launch_bounds__(T)
-preference_stats_rows(Rows<DT> r, const int32_t* __restrict__ seq_starts, int seqs, float* __restrict__ logp,
-                      float* __restrict__ row_max, float* __restrict__ row_sum, float* __restrict__ coef) {
-    __shared__ MaxSum s_red[T / 32];
-    const int row = blockIdx.x;
+// ---------------------------------------------------------------- longer rows: streamed
+// A row is cut into parts by its length alone, up to kMaxParts of them; a cluster of C blocks shares it, `per_block`
+// parts each.  Every part has its own maximum and sum, and they are merged in one order whatever C is: a row's
+// log-probability is the same number in every batch and in every operator.
+//
+// The gradient reads the row again.  The blocks that are resident at once hold 64 KB of logits each, 57 MB in all, so
+// that the second read comes from L2.
+constexpr int kStreamThreads = 256, kStreamWarps = kStreamThreads / 32;
+constexpr int kMaxParts = 8;
+constexpr int kPartVecs = 2048;             // 32 KB, unless the row has more than kMaxParts of them
+
+template <int DT, class P>
+__global__ void __launch_bounds__(kStreamThreads, 6)
+rows_streamed(Rows<DT> r, P p, int C, int parts, int per_block, int part_vecs) {
+    using L = Logit<DT>;
+    constexpr int T = kStreamThreads;
+    __shared__ MaxSum s_red[kMaxParts][kStreamWarps], s_parts[kMaxParts];
+    __shared__ Slope s_slope;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / C, rank = blockIdx.x - row * C;
+    ptx::wait_prior_grid();
+    ptx::let_next_grid_start();
     const int y = r.labels[row];
-    const bool counts = (unsigned)y < (unsigned)r.classes && row >= seq_starts[0] && row < seq_starts[seqs];
-    const auto* z = r.z + (int64_t)row * r.z_stride;
-    MaxSum a{0.f, 0.f};
-    if (counts) a = row_stats<DT, T>(z, r.classes, s_red);
-    if (threadIdx.x == 0) {
-        logp[row] = a.s != 0.f ? label_logp<DT>(z, y, a) : 0.f;
-        row_max[row] = a.m;
-        row_sum[row] = a.s;                                     // 0: the row does not count
-        coef[row] = 0.f;
+    const auto* z = r.logits(row);
+    if ((unsigned)y >= (unsigned)r.classes || !p.counts(row)) {     // the same in all blocks of the row
+        if (tid == 0 && rank == 0) p.skip(row);
+        if constexpr (P::kGradient) zero_row<DT, T>(r.gradient(row), r.classes, tid, rank, C);
+        return;
+    }
+    if (C > 1) ptx::cluster_arrive();
+    const RowSplit sp(z, r.classes);
+    const int part0 = rank * per_block, own = max(0, min(per_block, parts - part0));
+    // the last part takes a vector more or less as the row's alignment has it
+    auto part_end = [&](int q) { return q == parts - 1 ? sp.nvec : min(sp.nvec, (q + 1) * part_vecs); };
+    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
+    const int edge_at = rank == 0 ? sp.single(tid, r.classes) : -1;
+    for (int q = 0; q < own; ++q) {
+        Running run;
+        const int end = part_end(part0 + q);
+        int v = (part0 + q) * part_vecs + tid;
+        for (; v + 3 * T < end; v += 4 * T) {
+            const uint4 x[4] = {zv[v], zv[v + T], zv[v + 2 * T], zv[v + 3 * T]};
+            run.template take<DT>(x);
+        }
+        if (v < end) {
+            uint4 x[3];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                x[k] = make_uint4(Vec<DT>::kLow, Vec<DT>::kLow, Vec<DT>::kLow, Vec<DT>::kLow);
+                if (v + k * T < end) x[k] = zv[v + k * T];
+            }
+            run.template take<DT>(x);
+        }
+        if (part0 + q == 0 && edge_at >= 0) run.take_one(L::load(z + edge_at));
+        const MaxSum a = warp_merge<32>(run.total());
+        if (lane == 0) s_red[q][warp] = a;
+    }
+    typename P::In in{};
+    float zy = 0.f;
+    if (tid == 0) {
+        in = p.in(row);
+        zy = L::load(z + y);
+    }
+    __syncthreads();
+    MaxSum a{kFloor, 0.f};                                      // in lane q of warp 0: of the block's part q
+    if (warp == 0) {
+        for (int q = 0; q < own; ++q) {
+            const MaxSum b = warp_merge<kStreamWarps>(s_red[q][lane & (kStreamWarps - 1)]);
+            if (lane == q) a = b;
+        }
+    }
+    const int at = lane & (kMaxParts - 1);
+    if (C == 1) {
+        if (warp == 0) a = warp_merge<kMaxParts>({__shfl_sync(0xffffffffu, a.m, at), __shfl_sync(0xffffffffu, a.s, at)});
+    } else {
+        // every block writes its parts into every peer; the barrier passed first says that the peers run
+        ptx::cluster_wait();
+        if (warp == 0 && lane < own)
+            for (int peer = 0; peer < C; ++peer) {
+                const uint32_t to = ptx::map_to_cta(ptx::smem_u32(s_parts + part0 + lane), peer);
+                ptx::st_remote_u32(to, __float_as_uint(a.m));
+                ptx::st_remote_u32(to + 4, __float_as_uint(a.s));
+            }
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+        if (warp == 0) a = warp_merge<kMaxParts>(at < parts ? s_parts[at] : MaxSum{kFloor, 0.f});
+    }
+    if (tid == 0) {
+        const float coef = plain(a.m) ? p.finish(row, in, zy, a, rank == 0) : 0.f;
+        s_slope = P::kGradient ? slope_of(a, coef) : Slope{a.m, a.s, coef, 0.f};
+    }
+    __syncthreads();
+    const Slope g = s_slope;
+    auto* d = r.gradient(row);
+    if (!plain(g.m)) {                                          // seldom: every block takes the whole row
+        a = row_stats<DT, T>(z, r.classes, s_red[0]);
+        if (tid == 0) s_slope.coef = p.finish(row, in, zy, a, rank == 0);
+        __syncthreads();
+        if constexpr (P::kGradient) {
+            const float coef = s_slope.coef;
+            if (coef == 0.f) zero_row<DT, T>(d, r.classes, tid, rank, C);
+            else if (rank == 0) row_gradient<DT, T>(z, d, r.classes, y, a, coef);
+        }
+    } else if constexpr (P::kGradient) {
+        if (g.coef == 0.f) {
+            zero_row<DT, T>(d, r.classes, tid, rank, C);
+            return;
+        }
+        auto* dv = d + sp.head;
+        const bool wide = (reinterpret_cast<uintptr_t>(dv) & 15u) == 0;
+        const int begin = part0 * part_vecs, end = own > 0 ? part_end(part0 + own - 1) : 0;
+        auto sweep = [&](auto negative) {
+            constexpr bool kNeg = decltype(negative)::value;
+            int v = begin + tid;
+            if (wide) {
+                uint4* o = reinterpret_cast<uint4*>(dv);
+                for (; v + 3 * T < end; v += 4 * T) {
+                    const uint4 x[4] = {__ldcs(zv + v), __ldcs(zv + v + T), __ldcs(zv + v + 2 * T), __ldcs(zv + v + 3 * T)};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) __stcs(o + v + k * T, slope_vec<DT, kNeg>(x[k], g));
+                }
+                for (; v < end; v += T) __stcs(o + v, slope_vec<DT, kNeg>(__ldcs(zv + v), g));
+            } else {
+#pragma unroll 2
+                for (; v < end; v += T)
+                    store_any(dv + (int64_t)v * L::kVec, slope_vec<DT, kNeg>(__ldcs(zv + v), g), (int)sizeof(typename L::T));
+            }
+        };
+        if (g.coef > 0.f) sweep(std::true_type{});
+        else sweep(std::false_type{});
+        if (edge_at >= 0) L::store(d + edge_at, g.at(L::load(z + edge_at), edge_at == y));
+        // the label's element again, by the thread that stored its vector
+        const int vy = y < sp.head ? -1 : (y - sp.head) / L::kVec;
+        if (vy >= begin && vy < end && (vy - begin) % T == tid) L::store(d + y, g.at(L::load(z + y), true));
     }
 }
 
@@ -333,29 +692,45 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// Sequence sums, the pairs' losses and the rows' coefficients: one warp per pair, sums in double in a fixed order.
+// sum over the block's threads, in thread 0; `s_part` holds T / 32 entries
+template <int T>
+__device__ __forceinline__ double block_sum(double v, double* s_part) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0;
+    if (threadIdx.x == 0)
+        for (int i = 0; i < T / 32; ++i) v += s_part[i];
+    return v;
+}
+
+// Sequence sums, the pairs' losses and the rows' coefficients: a block per pair, sums in double in a fixed order.
 // Sequence bounds come from device memory: they are clamped to the rows, whatever they say.
-__global__ void __launch_bounds__(1024)
-preference_pairs(const float* __restrict__ logp, const float* __restrict__ row_sum,
-                 const int32_t* __restrict__ seq_starts, const float* __restrict__ ref_logp,
-                 const float* __restrict__ scaling, double beta, double smoothing, int rows, int pairs,
-                 float* __restrict__ seq_logp, float* __restrict__ loss_partial, float* __restrict__ loss,
-                 float* __restrict__ coef) {
-    __shared__ double s_loss[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double mine = 0.0;
-    for (int p = warp; p < pairs; p += 32) {
-        double sums[2];
-        int lo[2], hi[2];
+constexpr int kPairThreads = 256;
+
+__global__ void __launch_bounds__(kPairThreads)
+preference_pairs(const float* logp, const float* row_sum, const int32_t* seq_starts, const float* ref_logp,
+                 const float* scaling, double beta, double smoothing, int rows, int pairs, float* seq_logp,
+                 float* loss_partial, float* coef) {
+    __shared__ double s_part[kPairThreads / 32];
+    __shared__ float s_pull;
+    const int p = blockIdx.x;
+    ptx::wait_prior_grid();
+    ptx::let_next_grid_start();
+    int lo[2], hi[2];
+    double sums[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            lo[k] = min(max(seq_starts[2 * p + k], 0), rows);
-            hi[k] = min(max(seq_starts[2 * p + k + 1], 0), rows);
-            double t = 0.0;
-            for (int i = lo[k] + lane; i < hi[k]; i += 32) t += (double)logp[i];
-            sums[k] = warp_sum(t);
-            if (lane == 0) seq_logp[2 * p + k] = (float)sums[k];
-        }
+    for (int k = 0; k < 2; ++k) {
+        lo[k] = min(max(seq_starts[2 * p + k], 0), rows);
+        hi[k] = min(max(seq_starts[2 * p + k + 1], 0), rows);
+        double t = 0.0;
+        for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads) t += (double)logp[i];
+        sums[k] = block_sum<kPairThreads>(t, s_part);
+    }
+    if (threadIdx.x == 0) {
+        seq_logp[2 * p] = (float)sums[0];
+        seq_logp[2 * p + 1] = (float)sums[1];
         const double ref = ref_logp ? (double)ref_logp[2 * p] - (double)ref_logp[2 * p + 1] : 0.0;
         const double x = beta * (sums[0] - sums[1] - ref);
         // -log sigmoid(x) = max(-x, 0) + log1p(exp(-|x|)); sigmoid from the same exponential of a negative number
@@ -363,45 +738,92 @@ preference_pairs(const float* __restrict__ logp, const float* __restrict__ row_s
         const double up = x >= 0 ? 1.0 / (1.0 + tail) : tail / (1.0 + tail);        // sigmoid(x)
         const double down = x >= 0 ? tail / (1.0 + tail) : 1.0 / (1.0 + tail);      // sigmoid(-x)
         const double part = ((1.0 - smoothing) * (fmax(-x, 0.0) + soft) + smoothing * (fmax(x, 0.0) + soft)) / pairs;
-        const float pull = (float)(beta * (smoothing * up - (1.0 - smoothing) * down) / pairs * (double)scaling[0]);
-        if (lane == 0) loss_partial[p] = (float)(x == x ? part : x);
-        mine += x == x ? part : x;
+        loss_partial[p] = (float)(x == x ? part : x);
+        s_pull = (float)(beta * (smoothing * up - (1.0 - smoothing) * down) / pairs * (double)scaling[0]);
+    }
+    __syncthreads();
+    const float pull = s_pull;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-            for (int i = lo[k] + lane; i < hi[k]; i += 32)
-                if (row_sum[i] != 0.f) coef[i] = k ? -pull : pull;
-    }
-    if (lane == 0) s_loss[warp] = mine;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < 32; ++i) t += s_loss[i];
-        *loss = (float)t;
-    }
+    for (int k = 0; k < 2; ++k)
+        for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads)
+            if (row_sum[i] != 0.f) coef[i] = k ? -pull : pull;
 }
 
-template <int DT, int T>
-__global__ void __launch_bounds__(T)
-preference_gradient_rows(Rows<DT> r, const float* __restrict__ row_max, const float* __restrict__ row_sum,
-                         const float* __restrict__ coef) {
-    const int row = blockIdx.x;
-    row_gradient<DT, T>(r.z + (int64_t)row * r.z_stride, r.d + (int64_t)row * r.d_stride, r.classes, r.labels[row],
-                        row_max[row], row_sum[row], coef[row]);
-}
-
-// Sum of the rows' losses in double, in a fixed order.
-__global__ void __launch_bounds__(1024)
-row_loss_sum(const float* __restrict__ partial, int rows, float* __restrict__ loss) {
-    __shared__ double s_part[32];
+// Sum of the partial losses in double, in a fixed order, by one block of T threads.
+template <int T>
+__device__ __forceinline__ void sum_partials(const float* partial, int n, float* loss) {
+    __shared__ double s_part[T / 32];
     double t = 0.0;
-    for (int i = threadIdx.x; i < rows; i += 1024) t += (double)partial[i];
-    t = warp_sum(t);
-    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = t;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        t = warp_sum(s_part[threadIdx.x]);
-        if (threadIdx.x == 0) *loss = (float)t;
+    for (int i = threadIdx.x; i < n; i += T) t += (double)partial[i];
+    t = block_sum<T>(t, s_part);
+    if (threadIdx.x == 0) *loss = (float)t;
+}
+
+constexpr int kSumThreads = 512;
+
+__global__ void __launch_bounds__(kSumThreads)
+partial_loss_sum(const float* partial, int n, float* loss) {
+    ptx::wait_prior_grid();
+    sum_partials<kSumThreads>(partial, n, loss);
+}
+
+// Second pass of the preference loss: every row's maximum, sum and coef are known, nothing is left to wait for.  `parts`
+// blocks a row, a block's vectors in two batches of four loads a thread.  The first block also adds up the loss.
+constexpr int kSlopeThreads = 256, kSlopeVecs = 8 * kSlopeThreads;
+
+template <int DT>
+__global__ void __launch_bounds__(kSlopeThreads)
+preference_gradient_rows(Rows<DT> r, const float* row_max, const float* row_sum, const float* coef_of, int parts,
+                         const float* loss_partial, int pairs, float* loss) {
+    using L = Logit<DT>;
+    // from the last row down: what the first pass read last is still in L2
+    const int back = blockIdx.x / parts, part = blockIdx.x - back * parts, row = r.rows - 1 - back;
+    ptx::wait_prior_grid();
+    ptx::let_next_grid_start();
+    if (blockIdx.x == 0) sum_partials<kSlopeThreads>(loss_partial, pairs, loss);
+    const float coef = coef_of[row];
+    auto* d = r.gradient(row);
+    if (coef == 0.f) {
+        zero_row<DT, kSlopeThreads>(d, r.classes, threadIdx.x, part, parts);
+        return;
     }
+    const MaxSum a{row_max[row], row_sum[row]};
+    const int y = r.labels[row];
+    const auto* z = r.logits(row);
+    if (!plain(a.m)) {                                          // seldom
+        if (part == 0) row_gradient<DT, kSlopeThreads>(z, d, r.classes, y, a, coef);
+        return;
+    }
+    const RowSplit sp(z, r.classes);
+    const Slope g = slope_of(a, coef);
+    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
+    auto* dv = d + sp.head;
+    const bool wide = (reinterpret_cast<uintptr_t>(dv) & 15u) == 0, neg = coef > 0.f;
+#pragma unroll 1
+    for (int v0 = part * kSlopeVecs + threadIdx.x; v0 < sp.nvec; v0 += parts * kSlopeVecs)
+#pragma unroll
+    for (int b = 0; b < 8; b += 4) {
+        uint4 raw[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int v = v0 + (b + k) * kSlopeThreads;
+            if (v < sp.nvec) raw[k] = __ldcs(zv + v);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int v = v0 + (b + k) * kSlopeThreads;
+            if (v >= sp.nvec) continue;
+            const uint4 out = neg ? slope_vec<DT, true>(raw[k], g) : slope_vec<DT, false>(raw[k], g);
+            if (wide) __stcs(reinterpret_cast<uint4*>(dv) + v, out);
+            else store_any(dv + (int64_t)v * L::kVec, out, (int)sizeof(typename L::T));
+        }
+    }
+    const int e = part == 0 ? sp.single(threadIdx.x, r.classes) : -1;
+    if (e >= 0) L::store(d + e, g.at(L::load(z + e), e == y));
+    // the label's element again, by the thread that stored its vector
+    const int vy = y < sp.head ? -1 : (y - sp.head) / L::kVec;
+    if (vy >= 0 && vy < sp.nvec && vy / kSlopeVecs % parts == part && vy % kSlopeThreads == (int)threadIdx.x)
+        L::store(d + y, g.at(L::load(z + y), true));
 }
 
 // ---------------------------------------------------------------- argument checks
@@ -440,10 +862,39 @@ int check_logits(const LogitArgs& a, bool gradient, const char* who) {
 template <int DT>
 Rows<DT> rows_of(const LogitArgs& a) {
     using T = typename Logit<DT>::T;
-    return {static_cast<const T*>(a.logits), a.logits_stride, static_cast<T*>(a.dlogits), a.dlogits_stride, a.labels, a.classes};
+    return {static_cast<const T*>(a.logits), a.logits_stride, static_cast<T*>(a.dlogits), a.dlogits_stride, a.labels, a.rows, a.classes};
+}
+
+// One kernel over the rows: up to 256 vectors of 16 bytes (2048 half classes) by a warp each, longer ones streamed.
+template <int DT, class P>
+int launch_rows(const Rows<DT>& r, const P& p, cudaStream_t s, const char* who) {
+    const int nvec = r.classes / Logit<DT>::kVec;
+    if (nvec <= 256) {
+        const int grid = (r.rows + kShortWarps - 1) / kShortWarps;
+        auto* kernel = nvec <= 32 ? rows_short<DT, 1, P> : (nvec <= 64 ? rows_short<DT, 2, P> : (nvec <= 128 ? rows_short<DT, 4, P> : rows_short<DT, 8, P>));
+        TRB_CUDA_TRY(launch_chained(kernel, grid, 32 * kShortWarps, 1, 0, s, r, p));
+    } else {
+        int parts = (nvec + kPartVecs - 1) / kPartVecs, part_vecs = kPartVecs;
+        if (parts > kMaxParts) {
+            parts = kMaxParts;
+            part_vecs = (nvec + kMaxParts - 1) / kMaxParts;
+        }
+        // Blocks a row.  A gradient: one for every two parts, for the second read (see rows_streamed; 4096 x 32000 and
+        // 8192 x 131072 bfloat16 take 88 and 747 us so, 102 and 835 us with one for each part, 88 and 914 us with one for
+        // all).  Otherwise one for all (6000 x 50021: 88 us, two blocks 103 us: the blocks of a cluster start and end
+        // together).  Where that leaves blocks of the GPU unused, as many as there are parts.
+        const int64_t resident = (int64_t)sm_count() * 6;
+        int C = 1;
+        while (C < parts && r.rows <= 0x7fffffff / (2 * C) && ((P::kGradient && 2 * C < parts) || r.rows * (int64_t)C < resident))
+            C *= 2;
+        TRB_CUDA_TRY(launch_chained(rows_streamed<DT, P>, r.rows * C, kStreamThreads, C, 0, s, r, p, C, parts, (parts + C - 1) / C, part_vecs));
+    }
+    TRB_LAUNCH_CHECK(who);
+    return TRB200_OK;
 }
 
 }  // namespace
+
 }  // namespace trb
 
 // calls LAUNCH(DT) for the storage type
@@ -461,12 +912,10 @@ extern "C" int trb200_token_logp(const void* logits, int64_t logits_stride, cons
     if (rc != TRB200_OK) return rc;
     if (rows == 0) return TRB200_OK;
     TRB_REQUIRE(logp, TRB200_ERR_INVALID_ARGUMENT, "token_logp: null pointer");
-#define TRB_LAUNCH(DT) \
-    trb::token_logp_rows<DT, 256><<<rows, 256, 0, trb::as_stream(stream)>>>(trb::rows_of<DT>(a), logp, lse)
+    const trb::LogpRows p{logp, lse};
+#define TRB_LAUNCH(DT) return trb::launch_rows<DT>(trb::rows_of<DT>(a), p, trb::as_stream(stream), "token_logp")
     TRB_BY_DTYPE(dtype, TRB_LAUNCH);
 #undef TRB_LAUNCH
-    TRB_LAUNCH_CHECK("token_logp_rows");
-    return TRB200_OK;
 }
 
 extern "C" int trb200_policy_loss_fused(const void* logits, int64_t logits_stride, const int32_t* actions,
@@ -487,14 +936,15 @@ extern "C" int trb200_policy_loss_fused(const void* logits, int64_t logits_strid
     const trb::PolicyArgs p{old_logp, kl_coef != 0.f ? ref_logp : nullptr, advantages, weights, scaling, 1.0f - clip_low,
                             1.0f + clip_high, kl_coef, rows ? 1.0f / (float)rows : 0.f};
     if (rows > 0) {
-#define TRB_LAUNCH(DT) \
-    trb::policy_loss_rows<DT, 256><<<rows, 256, 0, trb::as_stream(stream)>>>(trb::rows_of<DT>(a), p, logp, loss_partial)
+        const trb::PolicyRows rows_p{p, logp, loss_partial};
+        int rc2 = TRB200_OK;
+#define TRB_LAUNCH(DT) rc2 = trb::launch_rows<DT>(trb::rows_of<DT>(a), rows_p, trb::as_stream(stream), "policy_loss")
         TRB_BY_DTYPE(dtype, TRB_LAUNCH);
 #undef TRB_LAUNCH
-        TRB_LAUNCH_CHECK("policy_loss_rows");
+        if (rc2 != TRB200_OK) return rc2;
     }
-    trb::row_loss_sum<<<1, 1024, 0, trb::as_stream(stream)>>>(loss_partial, rows, loss);
-    TRB_LAUNCH_CHECK("row_loss_sum");
+    TRB_CUDA_TRY(trb::launch_chained(trb::partial_loss_sum, 1, trb::kSumThreads, 1, 0, trb::as_stream(stream), loss_partial, rows, loss));
+    TRB_LAUNCH_CHECK("partial_loss_sum");
     return TRB200_OK;
 }
 
@@ -524,21 +974,31 @@ extern "C" int trb200_preference_loss_fused(const void* logits, int64_t logits_s
     float* row_sum = row_max + rows;
     float* coef = row_sum + rows;
     if (rows > 0) {
-#define TRB_LAUNCH(DT)                                                                                               \
-    trb::preference_stats_rows<DT, 256><<<rows, 256, 0, s>>>(trb::rows_of<DT>(a), seq_starts, 2 * pairs, logp, row_max, \
-                                                             row_sum, coef)
+        const trb::PairRows p{seq_starts, 2 * pairs, logp, row_max, row_sum, coef};
+        int rc2 = TRB200_OK;
+#define TRB_LAUNCH(DT) rc2 = trb::launch_rows<DT>(trb::rows_of<DT>(a), p, s, "preference_loss statistics")
         TRB_BY_DTYPE(dtype, TRB_LAUNCH);
 #undef TRB_LAUNCH
-        TRB_LAUNCH_CHECK("preference_stats_rows");
+        if (rc2 != TRB200_OK) return rc2;
     }
-    trb::preference_pairs<<<1, 1024, 0, s>>>(logp, row_sum, seq_starts, ref_logp, scaling, beta, label_smoothing, rows,
-                                             pairs, seq_logp, loss_partial, loss, coef);
+    TRB_CUDA_TRY(trb::launch_chained(trb::preference_pairs, pairs, trb::kPairThreads, 1, 0, s, logp, row_sum, seq_starts, ref_logp,
+                                     scaling, beta, label_smoothing, rows, pairs, seq_logp, loss_partial, coef));
     TRB_LAUNCH_CHECK("preference_pairs");
+    if (rows == 0) {
+        TRB_CUDA_TRY(trb::launch_chained(trb::partial_loss_sum, 1, trb::kSumThreads, 1, 0, s, loss_partial, pairs, loss));
+        TRB_LAUNCH_CHECK("partial_loss_sum");
+    }
     if (rows > 0) {
-#define TRB_LAUNCH(DT) \
-    trb::preference_gradient_rows<DT, 256><<<rows, 256, 0, s>>>(trb::rows_of<DT>(a), row_max, row_sum, coef)
+        const int nvec = classes / (16 / trb::elem_size(dtype));
+        int parts = nvec <= trb::kSlopeVecs ? 1 : (nvec + trb::kSlopeVecs - 1) / trb::kSlopeVecs;
+        if (parts > 0x7fffffff / rows) parts = 0x7fffffff / rows;
+        cudaError_t err = cudaSuccess;
+#define TRB_LAUNCH(DT)                                                                                                \
+    err = trb::launch_chained(trb::preference_gradient_rows<DT>, rows * parts, trb::kSlopeThreads, 1, 0, s, trb::rows_of<DT>(a), \
+                              row_max, row_sum, coef, parts, loss_partial, pairs, loss)
         TRB_BY_DTYPE(dtype, TRB_LAUNCH);
 #undef TRB_LAUNCH
+        TRB_CUDA_TRY(err);
         TRB_LAUNCH_CHECK("preference_gradient_rows");
     }
     return TRB200_OK;

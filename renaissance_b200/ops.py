@@ -621,7 +621,7 @@ FLOAT_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 class _On:
-    """Where a call runs: the tensors' device, and `stream` or that device's current one.  Allocations made inside
+    """A call on another device than the current one, or on a stream of the caller's choice.  Allocations made inside
     belong to that stream; tensors of another stream are held back from reuse until the call's work is done."""
 
     def __init__(self, device, stream, tensors):
@@ -631,13 +631,11 @@ class _On:
             raise ValueError(f"the stream belongs to {self.stream.device}, the tensors to {device}")
         self.raw = self.stream.cuda_stream
         self.device, self.tensors = device, tensors
-        self.contexts = []
-
-    def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self.contexts.append(torch.cuda.device(self.device))
+        self.contexts = [torch.cuda.device(device)]
         if self.raw != self.current.cuda_stream:
             self.contexts.append(torch.cuda.stream(self.stream))
+
+    def __enter__(self):
         for c in self.contexts:
             c.__enter__()
         return self
@@ -649,6 +647,14 @@ class _On:
             for t in self.tensors:
                 if t is not None:
                     t.record_stream(self.stream)
+
+
+def _call_on(device, stream, tensors, call):
+    """call(raw stream) where the tensors are: at once on the current device's current stream, else inside _On."""
+    if stream is None and device.index == torch.cuda.current_device():
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
+    with _On(device, stream, tensors) as on:
+        return call(on.raw)
 
 
 def _logit_rows(t, name):
@@ -691,12 +697,15 @@ def token_logprobs(logits, labels, stream=None):
     n, k = logits.shape
     dev = logits.device
     labels_p = _vector(labels, n, torch.int32, "labels", dev)
-    with _On(dev, stream, (logits, labels)) as on:
+
+    def call(raw):
         logp = torch.empty(n, dtype=torch.float32, device=dev)
         lse = torch.empty(n, dtype=torch.float32, device=dev)
         check(_lib.load().trb200_token_logp(logits.data_ptr(), stride, labels_p, logp.data_ptr(), lse.data_ptr(), n, k,
-                                            FLOAT_CODE[logits.dtype], on.raw))
-    return dict(logp=logp, lse=lse)
+                                            FLOAT_CODE[logits.dtype], raw))
+        return dict(logp=logp, lse=lse)
+
+    return _call_on(dev, stream, (logits, labels), call)
 
 
 def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0.2, clip_high=0.2, ref_logp=None,
@@ -719,16 +728,20 @@ def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0
     scaling_p = _vector(scaling, 1, f32, "scaling", dev)
     ref_p = None if ref_logp is None else _vector(ref_logp, n, f32, "ref_logp", dev)
     weights_p = None if weights is None else _vector(weights, n, f32, "weights", dev)
-    with _On(dev, stream, (logits, actions, old_logp, advantages, scaling, ref_logp, weights, dlogits)) as on:
-        dlogits, dstride = _gradient_rows(dlogits, logits)
+    held = (logits, actions, old_logp, advantages, scaling, ref_logp, weights, dlogits)
+
+    def call(raw):
+        d, dstride = _gradient_rows(dlogits, logits)
         logp = torch.empty(n, dtype=f32, device=dev)
         part = torch.empty(n, dtype=f32, device=dev)
         loss = torch.empty(1, dtype=f32, device=dev)
         check(_lib.load().trb200_policy_loss_fused(
             logits.data_ptr(), stride, actions_p, old_p, ref_p, adv_p, weights_p, scaling_p, clip_low, clip_high, kl_coef,
-            dlogits.data_ptr(), dstride, logp.data_ptr(), part.data_ptr(), loss.data_ptr(), n, k,
-            FLOAT_CODE[logits.dtype], on.raw))
-    return dict(loss=loss, loss_partial=part, logp=logp, dlogits=dlogits)
+            d.data_ptr(), dstride, logp.data_ptr(), part.data_ptr(), loss.data_ptr(), n, k, FLOAT_CODE[logits.dtype],
+            raw))
+        return dict(loss=loss, loss_partial=part, logp=logp, dlogits=d)
+
+    return _call_on(dev, stream, held, call)
 
 
 def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.1, label_smoothing=0.0, dlogits=None,
@@ -754,8 +767,9 @@ def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.
     ref_p = None if ref_logp is None else _vector(ref_logp, seqs, f32, "ref_logp", dev)
     scaling_p = _vector(scaling, 1, f32, "scaling", dev)
     lib = _lib.load()
-    with _On(dev, stream, (logits, labels, seq_starts, ref_logp, scaling, dlogits)) as on:
-        dlogits, dstride = _gradient_rows(dlogits, logits)
+
+    def call(raw):
+        d, dstride = _gradient_rows(dlogits, logits)
         logp = torch.empty(n, dtype=f32, device=dev)
         per_seq = torch.empty(seqs, dtype=f32, device=dev)
         part = torch.empty(seqs // 2, dtype=f32, device=dev)
@@ -763,10 +777,12 @@ def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.
         ws_bytes = lib.trb200_preference_loss_workspace_bytes(n)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         check(lib.trb200_preference_loss_fused(
-            logits.data_ptr(), stride, labels_p, starts_p, ref_p, scaling_p, beta, label_smoothing, dlogits.data_ptr(),
+            logits.data_ptr(), stride, labels_p, starts_p, ref_p, scaling_p, beta, label_smoothing, d.data_ptr(),
             dstride, logp.data_ptr(), per_seq.data_ptr(), part.data_ptr(), loss.data_ptr(), n, seqs // 2, k,
-            FLOAT_CODE[logits.dtype], ws.data_ptr(), ws_bytes, on.raw))
-    return dict(loss=loss, loss_partial=part, seq_logp=per_seq, logp=logp, dlogits=dlogits)
+            FLOAT_CODE[logits.dtype], ws.data_ptr(), ws_bytes, raw))
+        return dict(loss=loss, loss_partial=part, seq_logp=per_seq, logp=logp, dlogits=d)
+
+    return _call_on(dev, stream, (logits, labels, seq_starts, ref_logp, scaling, dlogits), call)
 
 
 # --------------------------------------------------------------------------- AdamW over many tensors
@@ -828,6 +844,7 @@ class AdamWPlan:
                                           8 if eight else 32, host.data_ptr(), host.numel(), C.byref(self.desc)))
         self.image = host.to(self.device)
         self.desc.image = self.image.data_ptr()
+        self.desc_ref = C.byref(self.desc)
         self.tensors = lists
 
 
@@ -850,9 +867,12 @@ def adamw_step(plan, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, scaling=None, s
     held = (step, lr if lr_p else None, scaling, skip_flag)
     if stream is not None:
         held += (plan.image, *(t for ts in plan.tensors.values() for t in ts))
-    with _On(dev, stream, held) as on:
-        check(_lib.load().trb200_adamw_step(C.byref(plan.desc), step_p, lr_v, lr_p, beta1, beta2, eps, scaling_p, skip_p,
-                                            seed, on.raw))
+
+    def call(raw):
+        check(_lib.load().trb200_adamw_step(plan.desc_ref, step_p, lr_v, lr_p, beta1, beta2, eps, scaling_p, skip_p, seed,
+                                            raw))
+
+    _call_on(dev, stream, held, call)
 
 
 # --------------------------------------------------------------------------- classifier

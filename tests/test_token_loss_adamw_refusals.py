@@ -93,10 +93,10 @@ def write(lib, tensors, grad=2, copy=-1, bits=32, short=0, null_image=False):
     return rc, desc
 
 
-def test_adamw_plan_counts_its_chunks(lib):
+def test_adamw_plan_counts_its_units(lib):
     rc, desc = write(lib, [tensor(1), tensor(0, 0x1100000), tensor(4097, 0x2100000)], copy=0, bits=8)
     assert rc == 0
-    assert (desc.count, desc.chunks, desc.grad_dtype, desc.copy_dtype, desc.state_bits) == (3, 3, 2, 0, 8)
+    assert (desc.count, desc.units, desc.grad_dtype, desc.copy_dtype, desc.state_bits) == (3, 1 + 0 + 17, 2, 0, 8)
     assert write(lib, [])[0] == 0
 
 
@@ -151,7 +151,7 @@ def test_adamw_step_refuses(lib):
     for kw in (dict(step=None), dict(lr=float("inf")), dict(b1=1.0), dict(b1=-0.1), dict(b2=1.0), dict(b2=float("nan")),
                dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan"))):
         assert step(**kw) == _lib.ERR_INVALID_ARGUMENT, kw
-    for field, value in (("image", None), ("image", 0x700008), ("count", -1), ("chunks", -1), ("grad_dtype", 5),
+    for field, value in (("image", None), ("image", 0x700008), ("count", -1), ("units", -1), ("grad_dtype", 5),
                          ("copy_dtype", 2), ("state_bits", 0)):
         bad = _lib.AdamWPlanDesc.from_buffer_copy(good)
         setattr(bad, field, value)

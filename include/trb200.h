@@ -361,7 +361,8 @@ int trb200_policy_loss_fused(const void* logits, int64_t logits_stride, const in
  * [2 * pairs] are written too.  Rows in front of seq_starts[0] and behind
  * seq_starts[2 * pairs] - 1 do not count.  Bounds outside [0, rows] are clamped; bounds
  * that do not ascend give wrong sums but no access outside the buffers.
- * workspace: trb200_preference_loss_workspace_bytes(rows), no contents expected. */
+ * workspace: trb200_preference_loss_workspace_bytes(rows), 8-byte aligned, no contents
+ * expected. */
 size_t trb200_preference_loss_workspace_bytes(int32_t rows);
 int trb200_preference_loss_fused(const void* logits, int64_t logits_stride, const int32_t* labels,
                                  const int32_t* seq_starts, const float* ref_logp, const float* scaling, double beta,

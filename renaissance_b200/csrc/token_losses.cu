@@ -337,8 +337,8 @@ struct Rows {
     __device__ __forceinline__ T* gradient(int row) const { return d + (int64_t)row * d_stride; }
 };
 
-// log-probability of the label with logit zy; never above 0
-__device__ __forceinline__ float label_logp(float zy, MaxSum a) { return (zy - a.m) - logf(a.s); }
+// log-probability of the label with logit zy, never above 0; in double, as sequences add it up
+__device__ __forceinline__ double label_logp(float zy, MaxSum a) { return ((double)zy - (double)a.m) - log((double)a.s); }
 
 // Each purpose says which rows count, takes a counting row's MaxSum to its outputs and, for a gradient, to coef.
 struct LogpRows {
@@ -355,7 +355,7 @@ struct LogpRows {
     __device__ __forceinline__ float finish(int row, const In&, float zy, MaxSum a, bool write) const {
         if (write) {
             const bool none = a.s == 0.f;                           // every logit is -inf
-            logp[row] = none ? -INFINITY : label_logp(zy, a);
+            logp[row] = none ? -INFINITY : (float)label_logp(zy, a);
             if (lse) lse[row] = none ? -INFINITY : a.m + logf(a.s);
         }
         return 0.f;
@@ -374,7 +374,7 @@ struct PolicyRows {
     __device__ __forceinline__ float finish(int row, const In& x, float zy, MaxSum a, bool write) const {
         float lp = 0.f, loss = 0.f, coef = 0.f;
         if (a.s != 0.f) {
-            lp = label_logp(zy, a);
+            lp = (float)label_logp(zy, a);
             policy_row(p, x, lp, loss, coef);
         }
         if (write) {
@@ -391,16 +391,22 @@ struct PairRows {
     const int32_t* seq_starts;
     int seqs;
     float* logp;
+    double* logp64;                 // what the sequence sums take: the float's rounding, 3e-7 a row, would add up
     float* row_max;
     float* row_sum;                 // 0: the row does not count
     float* coef;
     struct In {};
     __device__ __forceinline__ bool counts(int row) const { return row >= seq_starts[0] && row < seq_starts[seqs]; }
     __device__ __forceinline__ In in(int row) const { return {}; }
-    __device__ __forceinline__ void skip(int row) const { logp[row] = row_max[row] = row_sum[row] = coef[row] = 0.f; }
+    __device__ __forceinline__ void skip(int row) const {
+        logp[row] = row_max[row] = row_sum[row] = coef[row] = 0.f;
+        logp64[row] = 0.0;
+    }
     __device__ __forceinline__ float finish(int row, const In&, float zy, MaxSum a, bool write) const {
         if (write) {
-            logp[row] = a.s != 0.f ? label_logp(zy, a) : 0.f;
+            const double lp = a.s != 0.f ? label_logp(zy, a) : 0.0;
+            logp[row] = (float)lp;
+            logp64[row] = lp;
             row_max[row] = a.m;
             row_sum[row] = a.s;
             coef[row] = 0.f;
@@ -710,7 +716,7 @@ __device__ __forceinline__ double block_sum(double v, double* s_part) {
 constexpr int kPairThreads = 256;
 
 __global__ void __launch_bounds__(kPairThreads)
-preference_pairs(const float* logp, const float* row_sum, const int32_t* seq_starts, const float* ref_logp,
+preference_pairs(const double* logp, const float* row_sum, const int32_t* seq_starts, const float* ref_logp,
                  const float* scaling, double beta, double smoothing, int rows, int pairs, float* seq_logp,
                  float* loss_partial, float* coef) {
     __shared__ double s_part[kPairThreads / 32];
@@ -725,7 +731,7 @@ preference_pairs(const float* logp, const float* row_sum, const int32_t* seq_sta
         lo[k] = min(max(seq_starts[2 * p + k], 0), rows);
         hi[k] = min(max(seq_starts[2 * p + k + 1], 0), rows);
         double t = 0.0;
-        for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads) t += (double)logp[i];
+        for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads) t += logp[i];
         sums[k] = block_sum<kPairThreads>(t, s_part);
     }
     if (threadIdx.x == 0) {
@@ -949,7 +955,7 @@ extern "C" int trb200_policy_loss_fused(const void* logits, int64_t logits_strid
 }
 
 extern "C" size_t trb200_preference_loss_workspace_bytes(int32_t rows) {
-    return rows > 0 ? (size_t)rows * 3 * sizeof(float) : 0;
+    return rows > 0 ? (size_t)rows * (sizeof(double) + 3 * sizeof(float)) : 0;
 }
 
 extern "C" int trb200_preference_loss_fused(const void* logits, int64_t logits_stride, const int32_t* labels,
@@ -967,21 +973,22 @@ extern "C" int trb200_preference_loss_fused(const void* logits, int64_t logits_s
     TRB_REQUIRE(std::isfinite(beta) && label_smoothing >= 0.0 && label_smoothing <= 1.0, TRB200_ERR_INVALID_ARGUMENT,
                 "preference_loss: beta must be finite and label_smoothing lie in [0, 1]");
     TRB_REQUIRE(rows == 0 || (workspace && workspace_bytes >= trb200_preference_loss_workspace_bytes(rows) &&
-                              (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0),
+                              (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0),
                 TRB200_ERR_WORKSPACE, "preference_loss: workspace missing, too small or misaligned");
     cudaStream_t s = trb::as_stream(stream);
-    float* row_max = static_cast<float*>(workspace);
+    double* logp64 = static_cast<double*>(workspace);
+    float* row_max = reinterpret_cast<float*>(logp64 + rows);
     float* row_sum = row_max + rows;
     float* coef = row_sum + rows;
     if (rows > 0) {
-        const trb::PairRows p{seq_starts, 2 * pairs, logp, row_max, row_sum, coef};
+        const trb::PairRows p{seq_starts, 2 * pairs, logp, logp64, row_max, row_sum, coef};
         int rc2 = TRB200_OK;
 #define TRB_LAUNCH(DT) rc2 = trb::launch_rows<DT>(trb::rows_of<DT>(a), p, s, "preference_loss statistics")
         TRB_BY_DTYPE(dtype, TRB_LAUNCH);
 #undef TRB_LAUNCH
         if (rc2 != TRB200_OK) return rc2;
     }
-    TRB_CUDA_TRY(trb::launch_chained(trb::preference_pairs, pairs, trb::kPairThreads, 1, 0, s, logp, row_sum, seq_starts, ref_logp,
+    TRB_CUDA_TRY(trb::launch_chained(trb::preference_pairs, pairs, trb::kPairThreads, 1, 0, s, logp64, row_sum, seq_starts, ref_logp,
                                      scaling, beta, label_smoothing, rows, pairs, seq_logp, loss_partial, coef));
     TRB_LAUNCH_CHECK("preference_pairs");
     if (rows == 0) {

@@ -334,6 +334,31 @@ def test_preference_bounds_from_the_device_are_clamped():
     assert torch.equal(out["dlogits"], want["dlogits"]) and torch.equal(out["loss"], want["loss"])
 
 
+# ------------------------------------------------------------------------------------------------ one number for a row
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [100, 1000, 2048, 5001, 32000, 50021, 131072, 140000])
+def test_a_rows_logp_does_not_depend_on_batch_or_operator(dtype, classes):
+    """Few rows are cut among more thread blocks than many; the sums are the same ones, so that a ratio of the policy
+    with itself is exactly 1."""
+    from renaissance_b200 import ops
+    rows = 1500
+    z = rows_of(rows, classes, dtype, seed=classes)
+    y = ints(rows, classes)
+    w = torch.full((rows,), 1.0 / rows, device="cuda")
+    many = ops.token_logprobs(z, y)
+    for n in (1, 3, 100):
+        few = ops.token_logprobs(z[:n], y[:n])
+        assert torch.equal(few["logp"], many["logp"][:n]) and torch.equal(few["lse"], many["lse"][:n])
+    for n in (2, rows):
+        adv = floats(n, 5)
+        out = ops.policy_loss_fused(z[:n], y[:n], many["logp"][:n], adv, one(1.0), weights=w[:n])
+        assert torch.equal(out["logp"], many["logp"][:n])
+        assert torch.equal(out["loss_partial"], -adv * w[:n])           # ratio 1
+        st = torch.tensor([0, n // 2, n], dtype=torch.int32, device="cuda")
+        assert torch.equal(ops.preference_loss_fused(z[:n], y[:n], st, None, one(1.0))["logp"], many["logp"][:n])
+
+
 # ------------------------------------------------------------------------------------------------ how they are called
 
 def test_no_rows():

@@ -71,7 +71,7 @@ def test_preference_loss_needs_its_workspace(lib):
     assert lib.trb200_preference_loss_workspace_bytes(1000) >= 12000
     assert preference(lib, ws=None) == _lib.ERR_WORKSPACE
     assert preference(lib, ws_bytes=lib.trb200_preference_loss_workspace_bytes(4) - 1) == _lib.ERR_WORKSPACE
-    assert preference(lib, ws=E + 2) == _lib.ERR_WORKSPACE
+    assert preference(lib, ws=E + 4) == _lib.ERR_WORKSPACE
 
 
 # ------------------------------------------------------------------------------------------------ AdamW

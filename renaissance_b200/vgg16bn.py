@@ -13,7 +13,7 @@ reference's ``DeepLearningTask::run_train_epoch_gpu`` plays
     gradients: FC weights in float from their GEMM, conv weights half -> float per bucket (>= 50 MB, ending at
               tensor ends) in backward order, NCCL all-reduce
               per bucket overlapped with the rest of backward, non-finite check,
-              SGD with momentum on float master weights + half working copy
+              SGD with momentum (or AdamW, states in 32 or in 8 bits) on float master weights + half working copy
 
 Every kernel of the step runs in libtrb200.so: the named hot path (block backward,
 softmax-CE), the convolution forward, BN forward, pooling, casts, the optimizer, and the
@@ -74,7 +74,10 @@ def _fc_width(n):
 class Vgg16BnTrainer:
     def __init__(self, batch=256, image=224, classes=1000, lr=0.01, momentum=0.9, weight_decay=5e-4,
                  loss_scale=1024.0, label_smoothing=0.0, bucket_mb=50.0, seed=0, device=None,
-                 process_group=None, dropout=0.5, fc_width=4096, nccl_registered=None, bucket_plan="tensors"):
+                 process_group=None, dropout=0.5, fc_width=4096, nccl_registered=None, bucket_plan="tensors",
+                 optimizer="sgd", betas=(0.9, 0.999), eps=1e-8):
+        if optimizer not in ("sgd", "adamw", "adamw8"):
+            raise ValueError(f"optimizer: sgd, adamw or adamw8 expected, got {optimizer!r}")
         self.dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         self.batch, self.image, self.classes = batch, image, classes
         self.lr, self.beta, self.wd = lr, momentum, weight_decay
@@ -138,6 +141,8 @@ class Vgg16BnTrainer:
         self.w16 = torch.zeros(self.total, dtype=torch.float16, device=d)
         self.g16 = torch.zeros(self.half_numel - self.half_begin, dtype=torch.float16, device=d)
         self._init_params(seed)
+        self.betas, self.eps = betas, eps
+        self.adamw = None if optimizer == "sgd" else self._adamw_plan(8 if optimizer == "adamw8" else 32)
 
         # ---- buckets over the flat float gradient buffer, all-reduced as backward passes them
         self.buckets = GradientBuckets(
@@ -215,6 +220,36 @@ class Vgg16BnTrainer:
             return g32
         return torch.zeros(self.total, dtype=torch.float32, device=self.dev)
 
+    def _adamw_plan(self, bits):
+        """AdamW over the parameter slots: matrices decay, BN vectors and biases do not.  m32 is the first state of the
+        float form; the 8-bit form keeps codes and scales instead (zeros are zero states)."""
+        d = self.dev
+        cut = lambda buf: [buf[s.offset:s.offset + s.stored] for s in self.slots]
+        self.adamw_steps = torch.zeros(1, dtype=torch.int32, device=d)
+        scales = {}
+        if bits == 32:
+            self.v32 = torch.zeros(self.total, dtype=torch.float32, device=d)
+            m, v = cut(self.m32), cut(self.v32)
+            self.adamw_states = [self.m32, self.v32]
+        else:
+            self.m32 = None
+            m8, v8 = (torch.zeros(self.total, dtype=torch.uint8, device=d) for _ in range(2))
+            m, v = cut(m8.view(torch.float8_e4m3fn)), cut(v8.view(torch.float8_e4m3fn))
+            sizes = [-(-s.stored // ops.ADAMW_BLOCK) for s in self.slots]
+            flat = [torch.zeros(sum(sizes), dtype=torch.float32, device=d) for _ in range(2)]
+            scales = dict(m_scales=list(flat[0].split(sizes)), v_scales=list(flat[1].split(sizes)))
+            self.adamw_states = [m8, v8] + flat
+        return ops.AdamWPlan(cut(self.w32), cut(self.g32), m, v, copies=cut(self.w16),
+                             weight_decay=[self.wd if len(s.shape) > 1 else 0.0 for s in self.slots], **scales)
+
+    def _clear_states(self):
+        if self.adamw is None:
+            self.m32.zero_()
+        else:
+            self.adamw_steps.zero_()
+            for t in self.adamw_states:
+                t.zero_()
+
     def half_grad(self, slot: ParamSlot):
         """A conv weight's gradient in the half buffer (whose element 0 is flat element half_begin)."""
         o = slot.offset - self.half_begin
@@ -250,7 +285,7 @@ class Vgg16BnTrainer:
             self.view(self.w32, f["w"]).copy_(torch.from_numpy(p["w"]))
             self.view(self.w32, f["b"]).copy_(torch.from_numpy(p["b"]))
         self.w16.copy_(self.w32)
-        self.m32.zero_()
+        self._clear_states()
 
     def params(self):
         """Float master weights as numpy arrays (same structure as load_params takes)."""
@@ -366,15 +401,20 @@ class Vgg16BnTrainer:
         # ---- guard + optimizer over the whole flat range, then the loss-scale back-off (a step that saw a non-finite
         # gradient is skipped, halves the scale and resets the flag for the next step)
         ops.check_nonfinite(self.g32, self.nan_flag)
-        ops.sgd_momentum(self.w32, self.g32, self.m32, self.w16, self.lr, self.wd, self.beta,
-                         scaling=self.scaling, skip_flag=self.nan_flag)
+        if self.adamw is None:
+            ops.sgd_momentum(self.w32, self.g32, self.m32, self.w16, self.lr, self.wd, self.beta,
+                             scaling=self.scaling, skip_flag=self.nan_flag)
+        else:
+            ops.adamw_step(self.adamw, self.adamw_steps, self.lr, *self.betas, self.eps, scaling=self.scaling,
+                           skip_flag=self.nan_flag, seed=self.seed)
         ops.grad_scaling(self.nan_flag, self.scaling, clear_flag=True)
 
     def sync_weights_from_rank0(self):
-        """Every rank takes rank 0's master weights and momentum (after a diagnostic that let the ranks drift)."""
+        """Every rank takes rank 0's master weights and optimizer states (after a diagnostic that let the ranks drift)."""
         if self.world > 1:
             dist.broadcast(self.w32, src=0, group=self.pg)
-            dist.broadcast(self.m32, src=0, group=self.pg)
+            for t in [self.m32] if self.adamw is None else [self.adamw_steps] + self.adamw_states:
+                dist.broadcast(t, src=0, group=self.pg)
             self.w16.copy_(self.w32)
 
     def _end_of(self, group):

@@ -337,8 +337,8 @@ struct Rows {
     __device__ __forceinline__ T* gradient(int row) const { return d + (int64_t)row * d_stride; }
 };
 
-// log-probability of the label with logit zy, never above 0; in double, as sequences add it up
-__device__ __forceinline__ double label_logp(float zy, MaxSum a) { return ((double)zy - (double)a.m) - log((double)a.s); }
+// log-probability of the label with logit zy, never above 0
+__device__ __forceinline__ float label_logp(float zy, MaxSum a) { return (zy - a.m) - logf(a.s); }
 
 // Each purpose says which rows count, takes a counting row's MaxSum to its outputs and, for a gradient, to coef.
 struct LogpRows {
@@ -355,7 +355,7 @@ struct LogpRows {
     __device__ __forceinline__ float finish(int row, const In&, float zy, MaxSum a, bool write) const {
         if (write) {
             const bool none = a.s == 0.f;                           // every logit is -inf
-            logp[row] = none ? -INFINITY : (float)label_logp(zy, a);
+            logp[row] = none ? -INFINITY : label_logp(zy, a);
             if (lse) lse[row] = none ? -INFINITY : a.m + logf(a.s);
         }
         return 0.f;
@@ -374,7 +374,7 @@ struct PolicyRows {
     __device__ __forceinline__ float finish(int row, const In& x, float zy, MaxSum a, bool write) const {
         float lp = 0.f, loss = 0.f, coef = 0.f;
         if (a.s != 0.f) {
-            lp = (float)label_logp(zy, a);
+            lp = label_logp(zy, a);
             policy_row(p, x, lp, loss, coef);
         }
         if (write) {
@@ -391,7 +391,7 @@ struct PairRows {
     const int32_t* seq_starts;
     int seqs;
     float* logp;
-    double* logp64;                 // what the sequence sums take: the float's rounding, 3e-7 a row, would add up
+    double* logp64;                 // what the sequence sums take: the rounding of logp, 3e-7 a row, would add up
     float* row_max;
     float* row_sum;                 // 0: the row does not count
     float* coef;
@@ -404,9 +404,8 @@ struct PairRows {
     }
     __device__ __forceinline__ float finish(int row, const In&, float zy, MaxSum a, bool write) const {
         if (write) {
-            const double lp = a.s != 0.f ? label_logp(zy, a) : 0.0;
-            logp[row] = (float)lp;
-            logp64[row] = lp;
+            logp[row] = a.s != 0.f ? label_logp(zy, a) : 0.f;
+            logp64[row] = a.s != 0.f ? ((double)zy - (double)a.m) - log((double)a.s) : 0.0;
             row_max[row] = a.m;
             row_sum[row] = a.s;
             coef[row] = 0.f;
@@ -437,29 +436,31 @@ __device__ __forceinline__ MaxSum row_stats(const typename Logit<DT>::T* z, int 
     return block_merge<T>(a, s_red);
 }
 
-// zeros for the vectors [first, last) of a row and, for the block that is told so, its single elements
+// zeros for the row whose gradient is d, by `parts` groups of T threads
 template <int DT, int T>
 __device__ __forceinline__ void zero_row(typename Logit<DT>::T* d, int classes, int tid, int part, int parts) {
     const RowSplit sp(d, classes);
-    const int e = part == 0 ? sp.single(tid, classes) : -1;
-    if (e >= 0) Logit<DT>::store(d + e, 0.f);
+    if (part == 0)
+        for (int i = tid; i < sp.head + sp.tail; i += T) Logit<DT>::store(d + sp.single(i, classes), 0.f);
     uint4* dv = reinterpret_cast<uint4*>(d + sp.head);
 #pragma unroll 4
     for (int v = part * T + tid; v < sp.nvec; v += parts * T) __stcs(dv + v, make_uint4(0u, 0u, 0u, 0u));
 }
 
-// d = coef * ([c == y] - exp(z - m) / s) over the T threads of the block
+// d = coef * ([c == y] - exp(z - m) / s) by T threads
 template <int DT, int T>
 __device__ __forceinline__ void row_gradient(const typename Logit<DT>::T* z, typename Logit<DT>::T* d, int classes,
-                                             int y, MaxSum a, float coef) {
+                                             int y, MaxSum a, float coef, int tid) {
     using L = Logit<DT>;
     const RowSplit sp(z, classes);
     const float p = pivot(a.m), fall = -coef / a.s;
-    const int e = sp.single(threadIdx.x, classes);
-    if (e >= 0) L::store(d + e, fmaf(exp_of(L::load(z + e) - p), fall, e == y ? coef : 0.f));
+    for (int i = tid; i < sp.head + sp.tail; i += T) {
+        const int e = sp.single(i, classes);
+        L::store(d + e, fmaf(exp_of(L::load(z + e) - p), fall, e == y ? coef : 0.f));
+    }
     const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
 #pragma unroll 1
-    for (int v = threadIdx.x; v < sp.nvec; v += T) {
+    for (int v = tid; v < sp.nvec; v += T) {
         float f[L::kVec];
         L::unpack(zv[v], f);
         const int c0 = sp.head + v * L::kVec, jy = y - c0;
@@ -469,88 +470,110 @@ __device__ __forceinline__ void row_gradient(const typename Logit<DT>::T* z, typ
     }
 }
 
-// ---------------------------------------------------------------- short rows: one warp each, in registers
-constexpr int kShortWarps = 4;
+// ---------------------------------------------------------------- short rows: in registers
+// G lanes of a warp share a row, K vectors each; what a row costs beside its elements (setting up, merging, the loss
+// itself) is paid once for the 32 / G rows of the warp.
+constexpr int kShortThreads = 128;
 
-template <int DT, int K>
-__device__ __forceinline__ void store_slopes(const uint4 (&raw)[K], typename Logit<DT>::T* dv, int v0, int nvec, const Slope& g) {
-    constexpr int kVec = Logit<DT>::kVec;
-    const bool wide = (reinterpret_cast<uintptr_t>(dv) & 15u) == 0, neg = g.coef > 0.f;
+// The words are to be unpacked again by the next pass: kept as floats they would take twice the registers.
+template <int K>
+__device__ __forceinline__ void forget(uint4 (&raw)[K]) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int v = v0 + 32 * k;
-        if (v >= nvec) continue;
-        const uint4 out = neg ? slope_vec<DT, true>(raw[k], g) : slope_vec<DT, false>(raw[k], g);
-        if (wide) __stcs(reinterpret_cast<uint4*>(dv) + v, out);
-        else store_any(dv + (int64_t)v * kVec, out, (int)sizeof(typename Logit<DT>::T));
-    }
+    for (int k = 0; k < K; ++k) asm volatile("" : "+r"(raw[k].x), "+r"(raw[k].y), "+r"(raw[k].z), "+r"(raw[k].w));
 }
 
-template <int DT, int K, class P>
-__global__ void __launch_bounds__(32 * kShortWarps)
+// MaxSum of the plain path over the G lanes of a row, in all of them
+template <int G>
+__device__ __forceinline__ MaxSum group_merge(MaxSum a) {
+    float m = a.m;
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = a.s * exp_of(a.m - m);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return {m, s};
+}
+
+template <int DT, int G, int K, class P>
+__global__ void __launch_bounds__(kShortThreads, K >= 8 ? 5 : 8)
 rows_short(Rows<DT> r, P p) {
     using L = Logit<DT>;
-    const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * kShortWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & (G - 1);
+    const int row = blockIdx.x * (kShortThreads / G) + threadIdx.x / G;
     ptx::wait_prior_grid();
     ptx::let_next_grid_start();
-    if (row >= r.rows) return;
-    const int y = r.labels[row];
-    const auto* z = r.logits(row);
-    if ((unsigned)y >= (unsigned)r.classes || !p.counts(row)) {
-        if (lane == 0) p.skip(row);
-        if constexpr (P::kGradient) zero_row<DT, 32>(r.gradient(row), r.classes, lane, 0, 1);
-        return;
-    }
+    const bool there = row < r.rows;                            // lanes without a row, or with one that does not count,
+    const int y = there ? r.labels[row] : -1;                   // go along: the shuffles are the whole warp's
+    const bool counts = (unsigned)y < (unsigned)r.classes && p.counts(row);
+    const auto* z = r.logits(there ? row : 0);
     const RowSplit sp(z, r.classes);
     const uint4* zv = reinterpret_cast<const uint4*>(z + sp.head);
     uint4 raw[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         raw[k] = make_uint4(Vec<DT>::kLow, Vec<DT>::kLow, Vec<DT>::kLow, Vec<DT>::kLow);
-        if (lane + 32 * k < sp.nvec) raw[k] = __ldcs(zv + lane + 32 * k);
+        if (counts && lane + G * k < sp.nvec) raw[k] = __ldcs(zv + lane + G * k);
     }
-    const int edge_at = sp.single(lane, r.classes);
-    const float edge = edge_at >= 0 ? L::load(z + edge_at) : -INFINITY;
-    const auto in = p.in(row);
-    const float zy = L::load(z + y);
+    // single elements: fewer than 16 (half) or 8 (float) a row
+    constexpr int kEdges = (2 * L::kVec + G - 1) / G;
+    int edge_at[kEdges];
+    float edge[kEdges];
+#pragma unroll
+    for (int i = 0; i < kEdges; ++i) {
+        edge_at[i] = counts ? sp.single(lane + G * i, r.classes) : -1;
+        edge[i] = edge_at[i] >= 0 ? L::load(z + edge_at[i]) : -INFINITY;
+    }
+    typename P::In in{};
+    float zy = 0.f;
+    if (counts) {
+        in = p.in(row);
+        zy = L::load(z + y);
+    }
     Running run;
     run.template take<DT>(raw);
-    run.take_one(edge);
-    MaxSum a = warp_merge<32>(run.total());
-    if (!plain(a.m)) {                                          // seldom
+#pragma unroll
+    for (int i = 0; i < kEdges; ++i) run.take_one(edge[i]);
+    MaxSum a = group_merge<G>(run.total());
+    const bool ordinary = plain(a.m);
+    if (counts && !ordinary) {                                  // seldom: every lane takes the whole row
         a = {-INFINITY, 0.f};
-        if (edge_at >= 0) {
-            float f[1] = {edge};
+        for (int c = 0; c < r.classes; ++c) {
+            const float f[1] = {L::load(z + c)};
             take(a, f);
         }
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float f[L::kVec];
-            L::unpack(raw[k], f);
-            take(a, f);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            a = merge(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
     }
-    const float coef = p.finish(row, in, zy, a, lane == 0);     // the same in all lanes
+    if (!there) return;
+    if (!counts) {
+        if (lane == 0) p.skip(row);
+        if constexpr (P::kGradient) zero_row<DT, G>(r.gradient(row), r.classes, lane, 0, 1);
+        return;
+    }
+    const float coef = p.finish(row, in, zy, a, lane == 0);     // the same in all lanes of the row
     if constexpr (P::kGradient) {
         auto* d = r.gradient(row);
         if (coef == 0.f) {
-            zero_row<DT, 32>(d, r.classes, lane, 0, 1);
-        } else if (plain(a.m)) {
+            zero_row<DT, G>(d, r.classes, lane, 0, 1);
+        } else if (ordinary) {
             const Slope g = slope_of(a, coef);
             auto* dv = d + sp.head;
-            store_slopes<DT, K>(raw, dv, lane, sp.nvec, g);
-            if (edge_at >= 0) L::store(d + edge_at, g.at(edge, edge_at == y));
+            const bool wide = (reinterpret_cast<uintptr_t>(dv) & 15u) == 0, neg = coef > 0.f;
+            forget(raw);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int v = lane + G * k;
+                if (v >= sp.nvec) continue;
+                const uint4 out = neg ? slope_vec<DT, true>(raw[k], g) : slope_vec<DT, false>(raw[k], g);
+                if (wide) __stcs(reinterpret_cast<uint4*>(dv) + v, out);
+                else store_any(dv + v * L::kVec, out, (int)sizeof(typename L::T));
+            }
+#pragma unroll
+            for (int i = 0; i < kEdges; ++i)
+                if (edge_at[i] >= 0) L::store(d + edge_at[i], g.at(edge[i], edge_at[i] == y));
             // the label's element again, by the lane that stored its vector
             const int vy = (y - sp.head) / L::kVec;
-            if (y >= sp.head && vy < sp.nvec && (vy & 31) == lane) L::store(d + y, g.at(zy, true));
+            if (y >= sp.head && vy < sp.nvec && (vy & (G - 1)) == lane) L::store(d + y, g.at(zy, true));
         } else {
-            const float m = pivot(a.m), fall = -coef / a.s;
-            for (int c = lane; c < r.classes; c += 32)
-                L::store(d + c, fmaf(exp_of(L::load(z + c) - m), fall, c == y ? coef : 0.f));
+            row_gradient<DT, G>(z, d, r.classes, y, a, coef, lane);
         }
     }
 }
@@ -560,17 +583,18 @@ rows_short(Rows<DT> r, P p) {
 // parts each.  Every part has its own maximum and sum, and they are merged in one order whatever C is: a row's
 // log-probability is the same number in every batch and in every operator.
 //
-// The gradient reads the row again.  The blocks that are resident at once hold 64 KB of logits each, 57 MB in all, so
-// that the second read comes from L2.
-constexpr int kStreamThreads = 256, kStreamWarps = kStreamThreads / 32;
+// The gradient reads the row again.  The blocks that are resident at once (six of 256 threads an SM) hold 64 KB of logits
+// each, 57 MB in all, so that the second read comes from L2.  Shorter rows get smaller blocks: what a row costs beside its
+// elements is paid by every warp of its block.
+constexpr int kStreamThreads = 1536;         // of an SM, in blocks of 64, 128 or 256
 constexpr int kMaxParts = 8;
-constexpr int kPartVecs = 2048;             // 32 KB, unless the row has more than kMaxParts of them
+constexpr int kPartVecs = 4096;             // 64 KB, unless the row has more than kMaxParts of them
 
-template <int DT, class P>
-__global__ void __launch_bounds__(kStreamThreads, 6)
+template <int DT, int T, class P>
+__global__ void __launch_bounds__(T, kStreamThreads / T)
 rows_streamed(Rows<DT> r, P p, int C, int parts, int per_block, int part_vecs) {
     using L = Logit<DT>;
-    constexpr int T = kStreamThreads;
+    constexpr int kStreamWarps = T / 32;
     __shared__ MaxSum s_red[kMaxParts][kStreamWarps], s_parts[kMaxParts];
     __shared__ Slope s_slope;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -656,7 +680,7 @@ rows_streamed(Rows<DT> r, P p, int C, int parts, int per_block, int part_vecs) {
         if constexpr (P::kGradient) {
             const float coef = s_slope.coef;
             if (coef == 0.f) zero_row<DT, T>(d, r.classes, tid, rank, C);
-            else if (rank == 0) row_gradient<DT, T>(z, d, r.classes, y, a, coef);
+            else if (rank == 0) row_gradient<DT, T>(z, d, r.classes, y, a, coef, tid);
         }
     } else if constexpr (P::kGradient) {
         if (g.coef == 0.f) {
@@ -713,7 +737,7 @@ __device__ __forceinline__ double block_sum(double v, double* s_part) {
 
 // Sequence sums, the pairs' losses and the rows' coefficients: a block per pair, sums in double in a fixed order.
 // Sequence bounds come from device memory: they are clamped to the rows, whatever they say.
-constexpr int kPairThreads = 256;
+constexpr int kPairThreads = 1024;
 
 __global__ void __launch_bounds__(kPairThreads)
 preference_pairs(const double* logp, const float* row_sum, const int32_t* seq_starts, const float* ref_logp,
@@ -731,6 +755,7 @@ preference_pairs(const double* logp, const float* row_sum, const int32_t* seq_st
         lo[k] = min(max(seq_starts[2 * p + k], 0), rows);
         hi[k] = min(max(seq_starts[2 * p + k + 1], 0), rows);
         double t = 0.0;
+#pragma unroll 8
         for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads) t += logp[i];
         sums[k] = block_sum<kPairThreads>(t, s_part);
     }
@@ -750,9 +775,10 @@ preference_pairs(const double* logp, const float* row_sum, const int32_t* seq_st
     __syncthreads();
     const float pull = s_pull;
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-        for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads)
-            if (row_sum[i] != 0.f) coef[i] = k ? -pull : pull;
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll 8
+        for (int i = lo[k] + threadIdx.x; i < hi[k]; i += kPairThreads) coef[i] = row_sum[i] != 0.f ? (k ? -pull : pull) : 0.f;
+    }
 }
 
 // Sum of the partial losses in double, in a fixed order, by one block of T threads.
@@ -773,31 +799,34 @@ partial_loss_sum(const float* partial, int n, float* loss) {
     sum_partials<kSumThreads>(partial, n, loss);
 }
 
-// Second pass of the preference loss: every row's maximum, sum and coef are known, nothing is left to wait for.  `parts`
-// blocks a row, a block's vectors in two batches of four loads a thread.  The first block also adds up the loss.
-constexpr int kSlopeThreads = 256, kSlopeVecs = 8 * kSlopeThreads;
+// Second pass of the preference loss: every row's maximum, sum and coef are known, nothing is left to wait for.  G threads
+// a row, or G = all of the block's for each of the `parts` of a long one; a thread's vectors in batches of four loads.
+// The first block also adds up the loss.
+constexpr int kSlopeThreads = 256;
 
-template <int DT>
+template <int DT, int G>
 __global__ void __launch_bounds__(kSlopeThreads)
 preference_gradient_rows(Rows<DT> r, const float* row_max, const float* row_sum, const float* coef_of, int parts,
                          const float* loss_partial, int pairs, float* loss) {
     using L = Logit<DT>;
     // from the last row down: what the first pass read last is still in L2
-    const int back = blockIdx.x / parts, part = blockIdx.x - back * parts, row = r.rows - 1 - back;
+    const int tid = threadIdx.x & (G - 1), group = blockIdx.x * (kSlopeThreads / G) + threadIdx.x / G;
+    const int back = group / parts, part = group - back * parts, row = r.rows - 1 - back;
     ptx::wait_prior_grid();
     ptx::let_next_grid_start();
     if (blockIdx.x == 0) sum_partials<kSlopeThreads>(loss_partial, pairs, loss);
+    if (row < 0) return;
     const float coef = coef_of[row];
     auto* d = r.gradient(row);
     if (coef == 0.f) {
-        zero_row<DT, kSlopeThreads>(d, r.classes, threadIdx.x, part, parts);
+        zero_row<DT, G>(d, r.classes, tid, part, parts);
         return;
     }
     const MaxSum a{row_max[row], row_sum[row]};
     const int y = r.labels[row];
     const auto* z = r.logits(row);
     if (!plain(a.m)) {                                          // seldom
-        if (part == 0) row_gradient<DT, kSlopeThreads>(z, d, r.classes, y, a, coef);
+        if (part == 0) row_gradient<DT, G>(z, d, r.classes, y, a, coef, tid);
         return;
     }
     const RowSplit sp(z, r.classes);
@@ -806,30 +835,30 @@ preference_gradient_rows(Rows<DT> r, const float* row_max, const float* row_sum,
     auto* dv = d + sp.head;
     const bool wide = (reinterpret_cast<uintptr_t>(dv) & 15u) == 0, neg = coef > 0.f;
 #pragma unroll 1
-    for (int v0 = part * kSlopeVecs + threadIdx.x; v0 < sp.nvec; v0 += parts * kSlopeVecs)
+    for (int v0 = part * 8 * G + tid; v0 < sp.nvec; v0 += parts * 8 * G)
 #pragma unroll
-    for (int b = 0; b < 8; b += 4) {
-        uint4 raw[4];
+        for (int b = 0; b < 8; b += 4) {
+            uint4 raw[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int v = v0 + (b + k) * kSlopeThreads;
-            if (v < sp.nvec) raw[k] = __ldcs(zv + v);
+            for (int k = 0; k < 4; ++k)
+                if (v0 + (b + k) * G < sp.nvec) raw[k] = __ldcs(zv + v0 + (b + k) * G);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int v = v0 + (b + k) * G;
+                if (v >= sp.nvec) continue;
+                const uint4 out = neg ? slope_vec<DT, true>(raw[k], g) : slope_vec<DT, false>(raw[k], g);
+                if (wide) __stcs(reinterpret_cast<uint4*>(dv) + v, out);
+                else store_any(dv + (int64_t)v * L::kVec, out, (int)sizeof(typename L::T));
+            }
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int v = v0 + (b + k) * kSlopeThreads;
-            if (v >= sp.nvec) continue;
-            const uint4 out = neg ? slope_vec<DT, true>(raw[k], g) : slope_vec<DT, false>(raw[k], g);
-            if (wide) __stcs(reinterpret_cast<uint4*>(dv) + v, out);
-            else store_any(dv + (int64_t)v * L::kVec, out, (int)sizeof(typename L::T));
+    if (part == 0)
+        for (int i = tid; i < sp.head + sp.tail; i += G) {
+            const int e = sp.single(i, r.classes);
+            L::store(d + e, g.at(L::load(z + e), e == y));
         }
-    }
-    const int e = part == 0 ? sp.single(threadIdx.x, r.classes) : -1;
-    if (e >= 0) L::store(d + e, g.at(L::load(z + e), e == y));
     // the label's element again, by the thread that stored its vector
     const int vy = y < sp.head ? -1 : (y - sp.head) / L::kVec;
-    if (vy >= 0 && vy < sp.nvec && vy / kSlopeVecs % parts == part && vy % kSlopeThreads == (int)threadIdx.x)
-        L::store(d + y, g.at(L::load(z + y), true));
+    if (vy >= 0 && vy < sp.nvec && vy / (8 * G) % parts == part && vy % G == tid) L::store(d + y, g.at(L::load(z + y), true));
 }
 
 // ---------------------------------------------------------------- argument checks
@@ -850,7 +879,7 @@ int check_logits(const LogitArgs& a, bool gradient, const char* who) {
     TRB_REQUIRE(a.rows >= 0 && a.classes > 0 && a.logits_stride >= a.classes &&
                     (!gradient || a.dlogits_stride >= a.classes),
                 TRB200_ERR_INVALID_ARGUMENT, "%s: bad sizes (rows=%d classes=%d)", who, a.rows, a.classes);
-    TRB_REQUIRE(a.classes <= (1 << 30), TRB200_ERR_UNSUPPORTED, "%s: more than 2^30 classes", who);
+    TRB_REQUIRE(a.classes <= (1 << 30) && a.rows <= (1 << 30), TRB200_ERR_UNSUPPORTED, "%s: more than 2^30 rows or classes", who);
     if (a.rows == 0) return TRB200_OK;
     TRB_REQUIRE(a.logits && a.labels && (!gradient || a.dlogits), TRB200_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     const uintptr_t mask = (uintptr_t)elem_size(a.dtype) - 1;
@@ -871,29 +900,34 @@ Rows<DT> rows_of(const LogitArgs& a) {
     return {static_cast<const T*>(a.logits), a.logits_stride, static_cast<T*>(a.dlogits), a.dlogits_stride, a.labels, a.rows, a.classes};
 }
 
-// One kernel over the rows: up to 256 vectors of 16 bytes (2048 half classes) by a warp each, longer ones streamed.
+// One kernel over the rows.  Which one goes by their length alone, as do the sums in it.
 template <int DT, class P>
 int launch_rows(const Rows<DT>& r, const P& p, cudaStream_t s, const char* who) {
     const int nvec = r.classes / Logit<DT>::kVec;
     if (nvec <= 256) {
-        const int grid = (r.rows + kShortWarps - 1) / kShortWarps;
-        auto* kernel = nvec <= 32 ? rows_short<DT, 1, P> : (nvec <= 64 ? rows_short<DT, 2, P> : (nvec <= 128 ? rows_short<DT, 4, P> : rows_short<DT, 8, P>));
-        TRB_CUDA_TRY(launch_chained(kernel, grid, 32 * kShortWarps, 1, 0, s, r, p));
+        const int lanes = nvec <= 32 ? 8 : (nvec <= 128 ? 16 : 32);
+        const int grid = (int)(((int64_t)r.rows * lanes + kShortThreads - 1) / kShortThreads);
+        auto* kernel = nvec <= 8 ? rows_short<DT, 8, 1, P>
+                                 : (nvec <= 32 ? rows_short<DT, 8, 4, P>
+                                               : (nvec <= 64 ? rows_short<DT, 16, 4, P>
+                                                             : (nvec <= 128 ? rows_short<DT, 16, 8, P> : rows_short<DT, 32, 8, P>)));
+        TRB_CUDA_TRY(launch_chained(kernel, grid, kShortThreads, 1, 0, s, r, p));
     } else {
         int parts = (nvec + kPartVecs - 1) / kPartVecs, part_vecs = kPartVecs;
         if (parts > kMaxParts) {
             parts = kMaxParts;
             part_vecs = (nvec + kMaxParts - 1) / kMaxParts;
         }
-        // Blocks a row.  A gradient: one for every two parts, for the second read (see rows_streamed; 4096 x 32000 and
-        // 8192 x 131072 bfloat16 take 88 and 747 us so, 102 and 835 us with one for each part, 88 and 914 us with one for
-        // all).  Otherwise one for all (6000 x 50021: 88 us, two blocks 103 us: the blocks of a cluster start and end
-        // together).  Where that leaves blocks of the GPU unused, as many as there are parts.
-        const int64_t resident = (int64_t)sm_count() * 6;
+        // Blocks a row.  A gradient: one for each part, for the second read (see rows_streamed; 8192 x 131072 bfloat16 take
+        // 748 us so, 835 us with twice as many blocks and 914 us with one for the row).  Otherwise one for all parts
+        // (6000 x 50021: 92 us, two blocks 103 us: the blocks of a cluster start and end together), or one for each where
+        // that would leave blocks of the GPU unused.
+        const int T = nvec <= 1024 ? 64 : (nvec <= 2048 ? 128 : 256);
+        const int64_t resident = (int64_t)sm_count() * (kStreamThreads / T);
         int C = 1;
-        while (C < parts && r.rows <= 0x7fffffff / (2 * C) && ((P::kGradient && 2 * C < parts) || r.rows * (int64_t)C < resident))
-            C *= 2;
-        TRB_CUDA_TRY(launch_chained(rows_streamed<DT, P>, r.rows * C, kStreamThreads, C, 0, s, r, p, C, parts, (parts + C - 1) / C, part_vecs));
+        while (C < parts && r.rows <= 0x7fffffff / (2 * C) && (P::kGradient || r.rows * (int64_t)C < resident)) C *= 2;
+        auto* kernel = T == 64 ? rows_streamed<DT, 64, P> : (T == 128 ? rows_streamed<DT, 128, P> : rows_streamed<DT, 256, P>);
+        TRB_CUDA_TRY(launch_chained(kernel, r.rows * C, T, C, 0, s, r, p, C, parts, (parts + C - 1) / C, part_vecs));
     }
     TRB_LAUNCH_CHECK(who);
     return TRB200_OK;
@@ -997,12 +1031,17 @@ extern "C" int trb200_preference_loss_fused(const void* logits, int64_t logits_s
     }
     if (rows > 0) {
         const int nvec = classes / (16 / trb::elem_size(dtype));
-        int parts = nvec <= trb::kSlopeVecs ? 1 : (nvec + trb::kSlopeVecs - 1) / trb::kSlopeVecs;
+        // eight vectors a thread: 8 threads a row up to 64 vectors, 32 up to 512, then blocks of 2048 vectors each
+        const int G = nvec <= 64 ? 8 : (nvec <= 512 ? 32 : 256);
+        int parts = G < 256 ? 1 : (nvec + 2047) / 2048;
         if (parts > 0x7fffffff / rows) parts = 0x7fffffff / rows;
+        const unsigned grid = (unsigned)(((int64_t)rows * parts * G + trb::kSlopeThreads - 1) / trb::kSlopeThreads);
         cudaError_t err = cudaSuccess;
 #define TRB_LAUNCH(DT)                                                                                                \
-    err = trb::launch_chained(trb::preference_gradient_rows<DT>, rows * parts, trb::kSlopeThreads, 1, 0, s, trb::rows_of<DT>(a), \
-                              row_max, row_sum, coef, parts, loss_partial, pairs, loss)
+    auto* kernel = G == 8 ? trb::preference_gradient_rows<DT, 8>                                                      \
+                          : (G == 32 ? trb::preference_gradient_rows<DT, 32> : trb::preference_gradient_rows<DT, 256>); \
+    err = trb::launch_chained(kernel, grid, trb::kSlopeThreads, 1, 0, s, trb::rows_of<DT>(a), row_max, row_sum, coef, parts, \
+                              loss_partial, pairs, loss)
         TRB_BY_DTYPE(dtype, TRB_LAUNCH);
 #undef TRB_LAUNCH
         TRB_CUDA_TRY(err);

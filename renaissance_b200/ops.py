@@ -658,33 +658,37 @@ def _call_on(device, stream, tensors, call):
 
 
 def _logit_rows(t, name):
+    """(rows, classes, row stride) of a matrix of logits or of their gradient."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2):
         raise TypeError(f"{name}: 2-D CUDA tensor expected")
     if t.dtype not in FLOAT_CODE:
         raise TypeError(f"{name}: float16, bfloat16 or float32 expected, got {t.dtype}")
-    if t.shape[1] < 1 or max(t.shape) >= 1 << 31:
+    (n, k), (stride, unit) = t.shape, t.stride()
+    if not (0 < k < 1 << 31 and n < 1 << 31):
         raise ValueError(f"{name}: 1 to 2^31 - 1 classes and fewer than 2^31 rows expected")
-    stride = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-    if (t.stride(1) != 1 and t.shape[1] > 1) or stride < t.shape[1]:
+    if n <= 1:
+        stride = max(stride, k)
+    if (unit != 1 and k > 1) or stride < k:
         raise ValueError(f"{name}: unit column stride and rows that do not overlap expected (rows may be padded)")
-    return stride
+    return n, k, stride
 
 
 def _vector(t, n, dtype, name, device):
+    """Address of n consecutive elements."""
     if not (isinstance(t, torch.Tensor) and t.device == device):
         raise TypeError(f"{name}: tensor on {device} expected")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: dtype {dtype} expected, got {t.dtype}")
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name}: {n} consecutive elements expected, got shape {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _gradient_rows(dlogits, logits):
+def _gradient_rows(dlogits, logits, n, k):
     if dlogits is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
-    stride = _logit_rows(dlogits, "dlogits")
-    if dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+        return torch.empty_like(logits, memory_format=torch.contiguous_format), k
+    dn, dk, stride = _logit_rows(dlogits, "dlogits")
+    if (dn, dk) != (n, k) or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
         raise ValueError("dlogits: the logits' shape, type and device expected")
     return dlogits, stride
 
@@ -693,14 +697,13 @@ def token_logprobs(logits, labels, stream=None):
     """Log-probability of each row's label and the row's log-sum-exp: dict(logp, lse), float [rows].  logits [rows,
     classes] half, bfloat16 or float, labels int32.  A label outside [0, classes) gives 0 and 0 and its row is not
     read; a row of minus infinities gives -inf and -inf."""
-    stride = _logit_rows(logits, "logits")
-    n, k = logits.shape
+    n, k, stride = _logit_rows(logits, "logits")
     dev = logits.device
     labels_p = _vector(labels, n, torch.int32, "labels", dev)
 
     def call(raw):
         logp = torch.empty(n, dtype=torch.float32, device=dev)
-        lse = torch.empty(n, dtype=torch.float32, device=dev)
+        lse = torch.empty_like(logp)
         check(_lib.load().trb200_token_logp(logits.data_ptr(), stride, labels_p, logp.data_ptr(), lse.data_ptr(), n, k,
                                             FLOAT_CODE[logits.dtype], raw))
         return dict(logp=logp, lse=lse)
@@ -718,8 +721,7 @@ def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0
     weights default to 1 / rows (mask / mask.sum() for a mean over a mask).  Rows with weight 0 or an action outside
     [0, classes) do not count: zero gradient, logits not read.  `scaling` (device scalar) multiplies dlogits only.
     Returns dict(loss [1], loss_partial [rows], logp [rows], dlogits)."""
-    stride = _logit_rows(logits, "logits")
-    n, k = logits.shape
+    n, k, stride = _logit_rows(logits, "logits")
     dev = logits.device
     f32 = torch.float32
     actions_p = _vector(actions, n, torch.int32, "actions", dev)
@@ -731,10 +733,8 @@ def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0
     held = (logits, actions, old_logp, advantages, scaling, ref_logp, weights, dlogits)
 
     def call(raw):
-        d, dstride = _gradient_rows(dlogits, logits)
-        logp = torch.empty(n, dtype=f32, device=dev)
-        part = torch.empty(n, dtype=f32, device=dev)
-        loss = torch.empty(1, dtype=f32, device=dev)
+        d, dstride = _gradient_rows(dlogits, logits, n, k)
+        logp, part, loss = old_logp.new_empty(n), old_logp.new_empty(n), old_logp.new_empty(1)
         check(_lib.load().trb200_policy_loss_fused(
             logits.data_ptr(), stride, actions_p, old_p, ref_p, adv_p, weights_p, scaling_p, clip_low, clip_high, kl_coef,
             d.data_ptr(), dstride, logp.data_ptr(), part.data_ptr(), loss.data_ptr(), n, k, FLOAT_CODE[logits.dtype],
@@ -755,8 +755,7 @@ def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.
 
     ref_logp [2 * pairs]: the reference policy's S (None: 0).  Rows outside every sequence do not count (zero
     gradient).  Returns dict(loss [1], loss_partial [pairs], seq_logp [2 * pairs], logp [rows], dlogits)."""
-    stride = _logit_rows(logits, "logits")
-    n, k = logits.shape
+    n, k, stride = _logit_rows(logits, "logits")
     dev = logits.device
     f32 = torch.float32
     labels_p = _vector(labels, n, torch.int32, "labels", dev)
@@ -769,11 +768,9 @@ def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.
     lib = _lib.load()
 
     def call(raw):
-        d, dstride = _gradient_rows(dlogits, logits)
-        logp = torch.empty(n, dtype=f32, device=dev)
-        per_seq = torch.empty(seqs, dtype=f32, device=dev)
-        part = torch.empty(seqs // 2, dtype=f32, device=dev)
-        loss = torch.empty(1, dtype=f32, device=dev)
+        d, dstride = _gradient_rows(dlogits, logits, n, k)
+        logp, per_seq = scaling.new_empty(n), scaling.new_empty(seqs)
+        part, loss = scaling.new_empty(seqs // 2), scaling.new_empty(1)
         ws_bytes = lib.trb200_preference_loss_workspace_bytes(n)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         check(lib.trb200_preference_loss_fused(

@@ -42,8 +42,9 @@ def test_token_logp_refuses(lib, bad):
     assert b"token_logp" in lib.trb200_last_error()
 
 
-def test_too_many_classes_are_unsupported(lib):
+def test_too_many_rows_or_classes_are_unsupported(lib):
     assert logp(lib, stride=1 << 31, classes=(1 << 30) + 1) == _lib.ERR_UNSUPPORTED
+    assert logp(lib, rows=(1 << 30) + 1) == _lib.ERR_UNSUPPORTED
 
 
 @pytest.mark.parametrize("bad", [dict(z=None), dict(y=None), dict(old=None), dict(adv=None), dict(sc=None), dict(d=None),

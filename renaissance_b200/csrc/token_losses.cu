@@ -79,7 +79,7 @@ struct RowSplit {
         nvec = (classes - head) / kVec;
         tail = classes - head - nvec * kVec;
     }
-    // the single element of this thread, or -1 (head + tail < 2 * 16 / sizeof(T) <= 16 threads have one)
+    // single element `tid`, or -1 (there are head + tail, fewer than 2 * 16 / sizeof(T))
     __device__ __forceinline__ int single(int tid, int classes) const {
         if (tid < head) return tid;
         const int t = tid - head;
@@ -255,8 +255,8 @@ struct Running {
 };
 
 // What the gradient of a row needs: g_c = coef ([c == y] - exp(z_c - m) / s).  A 16-bit result is one multiply-add and
-// one exponential, |coef| p_c = 2^(z_c hi + up) with up = log2(|coef| / s) - m hi (within kPlain its rounding is 2^-15
-// of a power, next to the 2^-9 of the result's), and the sign is the conversion's.
+// one exponential, |coef| p_c = 2^(z_c hi + up) with up = log2(|coef| / s) - m hi (within kPlain its rounding is 2^-16
+// of the power, next to the 2^-12 or 2^-9 of the result's), and the sign is the conversion's.
 struct Slope {
     float m, s, coef, up;
     __device__ __forceinline__ float at(float z, bool label) const {        // one element in full precision

@@ -185,6 +185,34 @@ def test_captured_steps_follow_step_and_rate():
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_plans_on_two_streams_and_many_tensors(eight):
+    """Two plans of 700 tensors each step at once on two streams; the results are those of one after the other."""
+    from renaissance_b200 import ops
+    sizes = [1 + (i * 37) % 900 for i in range(697)] + [0, 300_000, 5]
+    sets = [tensors(sizes, torch.float16, torch.bfloat16, seed=s, eight=eight, started=False)[0] for s in (1, 2)]
+    want = [clone(t) for t in sets]
+    for t in want:
+        n = one(0, torch.int32)
+        p = plan_of(t, 0.1, eight)
+        for _ in range(3):
+            ops.adamw_step(p, n, LR, seed=5)
+    plans = [plan_of(t, 0.1, eight) for t in sets]
+    steps = [one(0, torch.int32) for _ in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for p, n, s in zip(plans, steps, streams):
+            ops.adamw_step(p, n, LR, seed=5, stream=s)
+    torch.cuda.synchronize()
+    bits = lambda x: x.view(torch.uint8) if x.element_size() == 1 else x
+    for got, ref, n in zip(sets, want, steps):
+        assert int(n) == 3
+        for k in ref:
+            for a, b in zip(got[k], ref[k]):
+                assert torch.equal(bits(a), bits(b)), k
+
+
 # ------------------------------------------------------------------------------------------------ 8-bit states
 
 def philox(counter, key):

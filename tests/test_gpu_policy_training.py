@@ -89,7 +89,7 @@ def test_policy_step_against_autograd(rows, features, classes, bits):
     loss = (rowloss * weights.double() * ok).sum()
     loss.backward()
     # logits: the GEMM's float sums, then half: one step of half where a sum sits next to a border (2^-10 of |z| < 8)
-    assert abs(float(out["loss"]) - float(loss)) < 2.0 ** -10 * 8
+    assert abs(float(out["loss"]) - float(loss.detach())) < 2.0 ** -10 * 8
     # d logits carry half a step of half each (2^-11), the products are summed in float: the gradient's norm by 2^-9
     gw, gb = head.gw.double() / 1024.0, head.gb.double() / 1024.0
     assert rel_l2(gw.cpu().numpy(), w.grad.cpu().numpy()) < 2.0 ** -8

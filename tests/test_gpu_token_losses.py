@@ -305,6 +305,20 @@ def test_preference_loss_far_apart_pairs_and_no_reference():
     assert not out["dlogits"].any()
 
 
+def test_preference_loss_many_pairs_and_long_sequences():
+    """2000 pairs of zero to three rows; two sequences of 20 000 rows."""
+    lens = [(i * 7) % 4 for i in range(4000)]
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    z = rows_of(starts[-1], 33, torch.bfloat16, seed=8)
+    check_preference(z, ints(starts[-1], 33), starts, floats(4000, 3, 2.0), 0.2, 0.1, 1e5)
+    z = rows_of(40_000, 17, torch.float32, seed=8)
+    y = ints(40_000, 17)
+    ref = torch.stack([stats64(z[:20_000], y[:20_000])[0].sum(), stats64(z[20_000:], y[20_000:])[0].sum()]).float()
+    check_preference(z, y, [0, 20_000, 40_000], ref, 0.1, 0.0, 1e3)
+
+
 def test_preference_rows_outside_and_without_distribution():
     from renaissance_b200 import ops
     z = rows_of(12, 500, torch.float16, seed=6)

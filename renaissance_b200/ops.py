@@ -620,7 +620,7 @@ def softmax_ce_amp_fused(logits, labels, scaling, label_smoothing, want_probs=Fa
 FLOAT_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-class _On:
+class _Elsewhere:
     """A call on another device than the current one, or on a stream of the caller's choice.  Allocations made inside
     belong to that stream; tensors of another stream are held back from reuse until the call's work is done."""
 
@@ -630,31 +630,28 @@ class _On:
         if self.stream.device != device:
             raise ValueError(f"the stream belongs to {self.stream.device}, the tensors to {device}")
         self.raw = self.stream.cuda_stream
-        self.device, self.tensors = device, tensors
+        self.tensors = tensors
         self.contexts = [torch.cuda.device(device)]
         if self.raw != self.current.cuda_stream:
             self.contexts.append(torch.cuda.stream(self.stream))
-
-    def __enter__(self):
         for c in self.contexts:
             c.__enter__()
-        return self
 
-    def __exit__(self, *exc):
+    def leave(self):
         for c in reversed(self.contexts):
-            c.__exit__(*exc)
+            c.__exit__(None, None, None)
         if self.raw != self.current.cuda_stream:
             for t in self.tensors:
                 if t is not None:
                     t.record_stream(self.stream)
 
 
-def _call_on(device, stream, tensors, call):
-    """call(raw stream) where the tensors are: at once on the current device's current stream, else inside _On."""
+def _where(device, stream, tensors):
+    """(raw stream, what to leave() after the call or None): where the tensors are, on `stream` or the current one."""
     if stream is None and device.index == torch.cuda.current_device():
-        return call(torch._C._cuda_getCurrentRawStream(device.index))
-    with _On(device, stream, tensors) as on:
-        return call(on.raw)
+        return torch._C._cuda_getCurrentRawStream(device.index), None
+    there = _Elsewhere(device, stream, tensors)
+    return there.raw, there
 
 
 def _logit_rows(t, name):
@@ -675,13 +672,13 @@ def _logit_rows(t, name):
 
 def _vector(t, n, dtype, name, device):
     """Address of n consecutive elements."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.numel() == n and t.device == device and t.is_contiguous():
+        return t.data_ptr()
     if not (isinstance(t, torch.Tensor) and t.device == device):
         raise TypeError(f"{name}: tensor on {device} expected")
     if t.dtype is not dtype:
         raise TypeError(f"{name}: dtype {dtype} expected, got {t.dtype}")
-    if t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name}: {n} consecutive elements expected, got shape {tuple(t.shape)}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: {n} consecutive elements expected, got shape {tuple(t.shape)}")
 
 
 def _gradient_rows(dlogits, logits, n, k):
@@ -700,15 +697,16 @@ def token_logprobs(logits, labels, stream=None):
     n, k, stride = _logit_rows(logits, "logits")
     dev = logits.device
     labels_p = _vector(labels, n, torch.int32, "labels", dev)
-
-    def call(raw):
+    raw, there = _where(dev, stream, (logits, labels))
+    try:
         logp = torch.empty(n, dtype=torch.float32, device=dev)
         lse = torch.empty_like(logp)
         check(_lib.load().trb200_token_logp(logits.data_ptr(), stride, labels_p, logp.data_ptr(), lse.data_ptr(), n, k,
                                             FLOAT_CODE[logits.dtype], raw))
         return dict(logp=logp, lse=lse)
-
-    return _call_on(dev, stream, (logits, labels), call)
+    finally:
+        if there:
+            there.leave()
 
 
 def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0.2, clip_high=0.2, ref_logp=None,
@@ -730,9 +728,8 @@ def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0
     scaling_p = _vector(scaling, 1, f32, "scaling", dev)
     ref_p = None if ref_logp is None else _vector(ref_logp, n, f32, "ref_logp", dev)
     weights_p = None if weights is None else _vector(weights, n, f32, "weights", dev)
-    held = (logits, actions, old_logp, advantages, scaling, ref_logp, weights, dlogits)
-
-    def call(raw):
+    raw, there = _where(dev, stream, (logits, actions, old_logp, advantages, scaling, ref_logp, weights, dlogits))
+    try:
         d, dstride = _gradient_rows(dlogits, logits, n, k)
         logp, part, loss = old_logp.new_empty(n), old_logp.new_empty(n), old_logp.new_empty(1)
         check(_lib.load().trb200_policy_loss_fused(
@@ -740,8 +737,9 @@ def policy_loss_fused(logits, actions, old_logp, advantages, scaling, clip_low=0
             d.data_ptr(), dstride, logp.data_ptr(), part.data_ptr(), loss.data_ptr(), n, k, FLOAT_CODE[logits.dtype],
             raw))
         return dict(loss=loss, loss_partial=part, logp=logp, dlogits=d)
-
-    return _call_on(dev, stream, held, call)
+    finally:
+        if there:
+            there.leave()
 
 
 def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.1, label_smoothing=0.0, dlogits=None,
@@ -766,8 +764,8 @@ def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.
     ref_p = None if ref_logp is None else _vector(ref_logp, seqs, f32, "ref_logp", dev)
     scaling_p = _vector(scaling, 1, f32, "scaling", dev)
     lib = _lib.load()
-
-    def call(raw):
+    raw, there = _where(dev, stream, (logits, labels, seq_starts, ref_logp, scaling, dlogits))
+    try:
         d, dstride = _gradient_rows(dlogits, logits, n, k)
         logp, per_seq = scaling.new_empty(n), scaling.new_empty(seqs)
         part, loss = scaling.new_empty(seqs // 2), scaling.new_empty(1)
@@ -778,8 +776,9 @@ def preference_loss_fused(logits, labels, seq_starts, ref_logp, scaling, beta=0.
             dstride, logp.data_ptr(), per_seq.data_ptr(), part.data_ptr(), loss.data_ptr(), n, seqs // 2, k,
             FLOAT_CODE[logits.dtype], ws.data_ptr(), ws_bytes, raw))
         return dict(loss=loss, loss_partial=part, seq_logp=per_seq, logp=logp, dlogits=d)
-
-    return _call_on(dev, stream, (logits, labels, seq_starts, ref_logp, scaling, dlogits), call)
+    finally:
+        if there:
+            there.leave()
 
 
 # --------------------------------------------------------------------------- AdamW over many tensors
@@ -864,12 +863,13 @@ def adamw_step(plan, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, scaling=None, s
     held = (step, lr if lr_p else None, scaling, skip_flag)
     if stream is not None:
         held += (plan.image, *(t for ts in plan.tensors.values() for t in ts))
-
-    def call(raw):
+    raw, there = _where(dev, stream, held)
+    try:
         check(_lib.load().trb200_adamw_step(plan.desc_ref, step_p, lr_v, lr_p, beta1, beta2, eps, scaling_p, skip_p, seed,
                                             raw))
-
-    _call_on(dev, stream, held, call)
+    finally:
+        if there:
+            there.leave()
 
 
 # --------------------------------------------------------------------------- classifier

@@ -512,3 +512,46 @@ def test_offsets_past_32_bits():
     pull = got["dlogits"][tail].double() / -(p - torch.nn.functional.one_hot(y[tail].long(), classes))
     at = pull.gather(1, y[tail].long()[:, None])
     assert (at.amax() - at.amin()) <= at.abs().amax() * 2.0 ** -7
+
+
+@pytest.mark.parametrize("classes", [1000, 33001])
+def test_captured_branches_that_join_before_a_loss(classes):
+    """One graph, two streams: the policy's and the reference's log-probabilities side by side, both waited for by the
+    loss, which begins while the kernel in front of it still runs.  Replays see new logits, as the same calls in a row
+    do."""
+    from renaissance_b200 import ops
+    rows = 300
+    z, y, old, adv, ref, w = policy_inputs(rows, classes, torch.bfloat16, 0, 0, 3, True, False)
+    other = rows_of(rows, classes, torch.bfloat16, seed=11)
+    scale = one(64.0)
+
+    def loss(side=None):
+        main = torch.cuda.current_stream()
+        if side is None:
+            was, before = ops.token_logprobs(z, y), ops.token_logprobs(other, y)
+        else:
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                before = ops.token_logprobs(other, y)
+            was = ops.token_logprobs(z, y)
+            main.wait_stream(side)
+        return ops.policy_loss_fused(z, y, was["logp"], adv, scale, 0.2, 0.28, before["logp"], 0.05)
+
+    loss()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = loss(side)
+    for step in range(5):
+        z.mul_(0.9)
+        other.add_(z)
+        for k in out:
+            out[k].fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want, apart = loss(), loss(torch.cuda.Stream())
+        torch.cuda.synchronize()
+        for k in out:
+            assert torch.equal(out[k].nan_to_num(), want[k].nan_to_num()), (k, step)
+            assert torch.equal(apart[k].nan_to_num(), want[k].nan_to_num()), (k, step)

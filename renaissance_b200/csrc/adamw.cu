@@ -14,8 +14,8 @@
 // becomes 0, which would make the update m / eps.
 //
 // Bound by HBM: 8 B of weight, the gradient, the copy and 16 B (float) or 4.125 B (8-bit) of state per element.  Float
-// states reach it: 138 M elements in 656 us, 0.97 of the copy bandwidth.  8-bit ones come near (486 us, 0.79; 25.6 M
-// elements with 16-bit gradients 87 us, 0.73): their 55 instructions an element (decoding, the update, the largest
+// states reach it: 138 M elements in 653 us, 0.97 of the copy bandwidth.  8-bit ones come near (488 us, 0.79; 25.6 M
+// elements with 16-bit gradients 87 us, 0.72): their 55 instructions an element (decoding, the update, the largest
 // magnitude of a block, random bits, encoding) take about as long as the bytes do, so that loads have to be on their way
 // all the time (asynchronous copies, three units ahead a warp) and pairs of floats go through the packed instructions.
 #include "chained.cuh"
@@ -629,8 +629,9 @@ extern "C" int trb200_adamw_step(const trb200_adamw_plan* plan, int32_t* step, f
     auto* head = reinterpret_cast<trb::Header*>(base);
     const auto* tensors = reinterpret_cast<const trb::Tensor*>(base + trb::tensors_at());
     const auto* units = reinterpret_cast<const int32_t*>(base + trb::units_at(plan->count));
-    // Three blocks an SM (float states: 655 us for 138 M elements against 690 with four, 710 with two).  Runs of 16 units
-    // (float) or 64 (8 bit), the same number for every block; small plans in runs that give every block something to do.
+    // Three blocks an SM (138 M elements, float states: 653 us against 690 with four, 710 with two; 8-bit ones 486 against
+    // 510 with four).  Runs of 16 units (float) or 64 (8 bit), the same number for every block; small plans in runs that
+    // give every block something to do.
     const bool e8 = plan->state_bits == 8;
     const int64_t resident = (int64_t)trb::sm_count() * 3, least = e8 ? trb::kWarps : 4, most = e8 ? 64 : 16;
     const int64_t rounds = (plan->units + resident * most - 1) / (resident * most);

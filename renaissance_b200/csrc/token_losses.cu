@@ -29,7 +29,7 @@ namespace trb {
 namespace {
 
 // log2(e) in two floats: with the first alone every exponent is 1.3e-8 of itself short, and log s, whose terms are all
-// off the same way, by 1.3e-7 at 100 000 classes (measured), which a sequence of 1000 rows adds up
+// off the same way, by 1.3e-7 at 131072 classes (measured; 3e-8 with both), which a sequence of 1000 rows adds up
 constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596303e-8f;
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -472,7 +472,11 @@ __device__ __forceinline__ void row_gradient(const typename Logit<DT>::T* z, typ
 
 // ---------------------------------------------------------------- short rows: in registers
 // G lanes of a warp share a row, K vectors each; what a row costs beside its elements (setting up, merging, the loss
-// itself) is paid once for the 32 / G rows of the warp.
+// itself) is paid once for the 32 / G rows of the warp: log-probabilities of 65536 rows of 64 bfloat16 classes take 6.4 us
+// with 8 lanes a row, 22.0 us with 32.  65536 x 1000 take 27.5 us (0.73 of the copy bandwidth), the policy loss 64.8 us.
+// Up to 2048 classes: 16383 x 1100 floats take 15.1 us (policy 39.6) here and 21.2 us (40.5) streamed.  Beyond, 16 bits,
+// 16384 x 4096: 23.9 us against 28.0, but the policy loss 59 us against 52.4, and all operators have to take the same
+// kernel for a length (see launch_rows).
 constexpr int kShortThreads = 128;
 
 // The words are to be unpacked again by the next pass: kept as floats they would take twice the registers.
@@ -495,7 +499,7 @@ __device__ __forceinline__ MaxSum group_merge(MaxSum a) {
 }
 
 template <int DT, int G, int K, class P>
-__global__ void __launch_bounds__(kShortThreads, K >= 8 ? 5 : 8)
+__global__ void __launch_bounds__(kShortThreads, K >= 16 ? 4 : (K >= 8 ? 5 : 8))
 rows_short(Rows<DT> r, P p) {
     using L = Logit<DT>;
     const int lane = threadIdx.x & (G - 1);
@@ -584,8 +588,14 @@ rows_short(Rows<DT> r, P p) {
 // log-probability is the same number in every batch and in every operator.
 //
 // The gradient reads the row again.  The blocks that are resident at once (six of 256 threads an SM) hold 64 KB of logits
-// each, 57 MB in all, so that the second read comes from L2.  Shorter rows get smaller blocks: what a row costs beside its
-// elements is paid by every warp of its block.
+// each, 57 MB in all, so that the second read comes from L2 (4096 x 32000 bfloat16: 269 MB are read from HBM, 262 MB of
+// logits).  Shorter rows get smaller blocks: what a row costs beside its elements is paid by every warp of its block
+// (log-probabilities, 16384 rows: 2056 classes 25.1 us with 64 threads, 56.9 us with 256; 4096 classes 28.0 and 60.1 us).
+//
+// Log-probabilities of 6000 x 50021: 91 us, 0.81 of the copy bandwidth.  Policy loss: 4096 x 32000, a quarter of the rows
+// masked, 86 us, 0.82; 8192 x 131072, a tenth masked, 756 us, 0.83.  At 4096 x 32000 with every row counting, 11.4
+// instructions a logit take 51 % of the issue slots and the exponentials 75 % of their unit; warps wait for loads and for
+// the block's barriers.  In a loop the GPU runs into its power limit at 8192 x 131072 (1000 W, 1.6 GHz).
 constexpr int kStreamThreads = 1536;         // of an SM, in blocks of 64, 128 or 256
 constexpr int kMaxParts = 8;
 constexpr int kPartVecs = 4096;             // 64 KB, unless the row has more than kMaxParts of them
@@ -736,7 +746,8 @@ __device__ __forceinline__ double block_sum(double v, double* s_part) {
 }
 
 // Sequence sums, the pairs' losses and the rows' coefficients: a block per pair, sums in double in a fixed order.
-// Sequence bounds come from device memory: they are clamped to the rows, whatever they say.
+// Sequence bounds come from device memory: they are clamped to the rows, whatever they say.  Bound by latency (10 us for
+// the one pair of 4096 rows; a warp a pair took 70 us).
 constexpr int kPairThreads = 1024;
 
 __global__ void __launch_bounds__(kPairThreads)
@@ -801,7 +812,9 @@ partial_loss_sum(const float* partial, int n, float* loss) {
 
 // Second pass of the preference loss: every row's maximum, sum and coef are known, nothing is left to wait for.  G threads
 // a row, or G = all of the block's for each of the `parts` of a long one; a thread's vectors in batches of four loads.
-// The first block also adds up the loss.
+// The first block also adds up the loss.  Bound by HBM: 4096 x 32000 bfloat16 take 81 us under the profiler, 473 MB at 71 %
+// of the DRAM's peak.  Groups of threads against a block a row (whole preference loss): 65536 x 64 31 us against 166 us,
+// 16384 x 4096 78 us against 102 us.
 constexpr int kSlopeThreads = 256;
 
 template <int DT, int G>
@@ -904,13 +917,15 @@ Rows<DT> rows_of(const LogitArgs& a) {
 template <int DT, class P>
 int launch_rows(const Rows<DT>& r, const P& p, cudaStream_t s, const char* who) {
     const int nvec = r.classes / Logit<DT>::kVec;
-    if (nvec <= 256) {
+    if (nvec <= 2048 / Logit<DT>::kVec) {
         const int lanes = nvec <= 32 ? 8 : (nvec <= 128 ? 16 : 32);
         const int grid = (int)(((int64_t)r.rows * lanes + kShortThreads - 1) / kShortThreads);
         auto* kernel = nvec <= 8 ? rows_short<DT, 8, 1, P>
                                  : (nvec <= 32 ? rows_short<DT, 8, 4, P>
                                                : (nvec <= 64 ? rows_short<DT, 16, 4, P>
                                                              : (nvec <= 128 ? rows_short<DT, 16, 8, P> : rows_short<DT, 32, 8, P>)));
+        if constexpr (DT == TRB200_DTYPE_F32)
+            if (nvec > 256) kernel = rows_short<DT, 32, 16, P>;
         TRB_CUDA_TRY(launch_chained(kernel, grid, kShortThreads, 1, 0, s, r, p));
     } else {
         int parts = (nvec + kPartVecs - 1) / kPartVecs, part_vecs = kPartVecs;
@@ -920,7 +935,7 @@ int launch_rows(const Rows<DT>& r, const P& p, cudaStream_t s, const char* who) 
         }
         // Blocks a row.  A gradient: one for each part, for the second read (see rows_streamed; 8192 x 131072 bfloat16 take
         // 748 us so, 835 us with twice as many blocks and 914 us with one for the row).  Otherwise one for all parts
-        // (6000 x 50021: 92 us, two blocks 103 us: the blocks of a cluster start and end together), or one for each where
+        // (6000 x 50021: 91 us, two blocks 103 us: the blocks of a cluster start and end together), or one for each where
         // that would leave blocks of the GPU unused.
         const int T = nvec <= 1024 ? 64 : (nvec <= 2048 ? 128 : 256);
         const int64_t resident = (int64_t)sm_count() * (kStreamThreads / T);

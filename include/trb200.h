@@ -615,7 +615,9 @@ int trb200_adamw_plan_write(const trb200_adamw_tensor* tensors, int32_t count, i
  * kernel, so that a captured step can be replayed; lr_dev (device scalar, may be NULL)
  * is used instead of lr.  Nothing at all happens if *skip_flag != 0 (the non-finite
  * guard; NULL = never).  scaling: device scalar, NULL = 1.  Steps of one plan must not
- * overlap one another.  0 <= beta < 1, eps > 0. */
+ * overlap one another.  0 <= beta < 1.  eps: at least 2^-55 / sqrt(1 - beta2) with float
+ * states (8.8e-16 for 0.999) and 2^-53 / sqrt(1 - beta2) with 8-bit ones (3.5e-15), below
+ * which what v loses where it is tiny would show in the update; at most 2^126. */
 int trb200_adamw_step(const trb200_adamw_plan* plan, int32_t* step, float lr, const float* lr_dev, double beta1,
                       double beta2, float eps, const float* scaling, const int32_t* skip_flag, uint64_t seed,
                       void* stream);

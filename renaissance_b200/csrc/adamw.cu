@@ -25,7 +25,6 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
-#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <type_traits>
@@ -113,12 +112,14 @@ __device__ __forceinline__ void moments(const Quad& g, Quad& m, Quad& v, const H
     v = {moment(v.a, mul2(g.a, g.a), h.beta2, h.rest2, h), moment(v.b, mul2(g.b, g.b), h.beta2, h.rest2, h)};
 }
 
-// Square root and reciprocal are the approximate ones, together good to 2^-21 of the change, which is a thousandth of the
-// weight or less: the weight's own rounding hides it.
+// Square root and reciprocal are the approximate ones, together good to 2^-21 of the change (the correctly rounded ones
+// would be two roundings, 2^-23, for several times the instructions): next to a weight well above lr the weight's own
+// rounding hides it, a weight that starts at 0 carries it.  The square root takes subnormal v as they are: flushed to
+// zero, v below 2^-126 would leave eps alone in the denominator.
 __device__ __forceinline__ uint64_t updated(uint64_t w, uint64_t m, uint64_t v, float decay, const Scalars& s, float eps) {
     float2 f = split(v);
-    asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(f.x));
-    asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+    asm("sqrt.approx.f32 %0, %0;" : "+f"(f.x));
+    asm("sqrt.approx.f32 %0, %0;" : "+f"(f.y));
     f = split(fma2(pair_of(f.x, f.y), twice(s.widen), twice(eps)));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.x));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.y));
@@ -508,6 +509,14 @@ Kernel kernel_of(int grad, int copy, bool e8) {
                                     : (grad == TRB200_DTYPE_F16 ? kernel_of<TRB200_DTYPE_F16>(copy, e8) : kernel_of<TRB200_DTYPE_BF16>(copy, e8));
 }
 
+// The smallest eps.  A float v is off by 2^-149 / (1 - beta2) at most where it is subnormal, whatever the step (each step
+// adds up to 2^-149, and the bias correction is at most 1 / (1 - beta2)), hence the root by 2^-74.5 / sqrt(1 - beta2):
+// 2^-19.5 of the smallest eps.  A block of an 8-bit v below kSmallest is stored as zeros, which takes
+// 2^-58 / sqrt(1 - beta2) from the root: 2^-5 of the smallest eps, half a step of the codes.  With a smaller eps the
+// denominator of such an element could come out as next to nothing, and its change as orders of magnitude too large.
+double least_eps(double beta2, bool e8) { return std::ldexp(1.0, e8 ? -53 : -55) / std::sqrt(1.0 - beta2); }
+constexpr float kMostEps = 8.50705917e37f;  // 2^126: the reciprocal of anything larger would be flushed to zero
+
 int64_t units_of(int64_t n) { return (n + kUnit - 1) / kUnit; }
 
 // units of all tensors, or -1 for a bad description
@@ -614,17 +623,20 @@ extern "C" int trb200_adamw_step(const trb200_adamw_plan* plan, int32_t* step, f
                                  double beta2, float eps, const float* scaling, const int32_t* skip_flag, uint64_t seed,
                                  void* stream) {
     TRB_REQUIRE(plan && plan->image && step, TRB200_ERR_INVALID_ARGUMENT, "adamw_step: null pointer");
-    TRB_REQUIRE((reinterpret_cast<uintptr_t>(plan->image) & 15u) == 0, TRB200_ERR_INVALID_ARGUMENT,
-                "adamw_step: the plan's image must be 16-byte aligned");
     TRB_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, TRB200_ERR_INVALID_ARGUMENT,
                 "adamw_step: beta1 and beta2 must lie in [0, 1)");
-    TRB_REQUIRE(eps >= FLT_MIN && std::isfinite(eps) && std::isfinite(lr), TRB200_ERR_INVALID_ARGUMENT,
-                "adamw_step: eps must be a positive normal float, lr finite");
+    TRB_REQUIRE(std::isfinite(lr), TRB200_ERR_INVALID_ARGUMENT, "adamw_step: lr must be finite");
     TRB_REQUIRE(plan->count >= 0 && plan->units >= 0 &&
                     (trb::valid_dtype(plan->grad_dtype) || plan->grad_dtype == TRB200_DTYPE_F32) &&
                     (trb::valid_dtype(plan->copy_dtype) || plan->copy_dtype == TRB200_DTYPE_NONE) &&
                     (plan->state_bits == 32 || plan->state_bits == 8),
                 TRB200_ERR_INVALID_ARGUMENT, "adamw_step: not a plan that trb200_adamw_plan_write wrote");
+    const bool e8 = plan->state_bits == 8;
+    TRB_REQUIRE(eps >= trb::least_eps(beta2, e8) && eps <= trb::kMostEps, TRB200_ERR_INVALID_ARGUMENT,
+                "adamw_step: eps = %g, but with beta2 = %.9g and %d-bit states it must lie in [%.3g, 8.5e37]", (double)eps, beta2,
+                (int)plan->state_bits, trb::least_eps(beta2, e8));
+    TRB_REQUIRE((reinterpret_cast<uintptr_t>(plan->image) & 15u) == 0, TRB200_ERR_INVALID_ARGUMENT,
+                "adamw_step: the plan's image must be 16-byte aligned");
     char* base = static_cast<char*>(plan->image);
     auto* head = reinterpret_cast<trb::Header*>(base);
     const auto* tensors = reinterpret_cast<const trb::Tensor*>(base + trb::tensors_at());
@@ -634,7 +646,6 @@ extern "C" int trb200_adamw_step(const trb200_adamw_plan* plan, int32_t* step, f
     // in runs that give every block something to do.  Float runs of 4 take 646 us for one tensor of 138 M elements (655), but
     // 127 us for 160 tensors of 160 000 (121.5); 8-bit ones of 8 take 107 us for 25.6 M elements (87), of 232, the same for
     // every block, 88.
-    const bool e8 = plan->state_bits == 8;
     const int64_t resident = (int64_t)trb::sm_count() * 3, least = e8 ? trb::kWarps : 4, most = e8 ? 64 : 16;
     const int64_t rounds = (plan->units + resident * most - 1) / (resident * most);
     int64_t run = rounds ? (plan->units + resident * rounds - 1) / (resident * rounds) : least;

@@ -852,7 +852,8 @@ def adamw_step(plan, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, scaling=None, s
 
     `step`: int32 device scalar, the steps taken so far; the kernel advances it, so a captured step can be replayed.
     `lr`: a number, or a float device scalar that a schedule writes between replays.  Nothing happens where the device
-    scalar `skip_flag` (int32) is not 0.  `seed` keys the stochastic rounding of 8-bit second moments."""
+    scalar `skip_flag` (int32) is not 0.  `seed` keys the stochastic rounding of 8-bit second moments.  `eps` has to be at
+    least 2^-55 / sqrt(1 - beta2) (8.8e-16 for 0.999), with 8-bit states four times that."""
     if not isinstance(plan, AdamWPlan):
         raise TypeError("adamw_step: an AdamWPlan expected")
     dev = plan.device

@@ -389,3 +389,76 @@ def test_plan_refuses_on_device():
         ops.adamw_step(plan, step, LR, beta1=1.0)
     with pytest.raises(_lib.Trb200Error):
         ops.adamw_step(plan, step, LR, eps=0.0)
+
+
+# ------------------------------------------------------------------------------------------------ tiny second moments
+
+def least_eps(beta2, eight):
+    return 2.0 ** (-53 if eight else -55) / math.sqrt(1 - beta2)
+
+
+def zero_states(g, eight, w=0.0):
+    n = g.numel()
+    state = lambda: torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) if eight else torch.zeros(n, device="cuda")
+    t = dict(w=[torch.full((n,), w, device="cuda")], g=[g], m=[state()], v=[state()], c=[])
+    if eight:
+        t["ms"], t["vs"] = ([torch.zeros(-(-n // 128), device="cuda")] for _ in range(2))
+    return t
+
+
+@pytest.mark.parametrize("beta2", [0.99, 0.999, 0.9999])
+@pytest.mark.parametrize("eight", [False, True])
+def test_first_step_with_tiny_gradients_and_eps(eight, beta2):
+    """v of the first step is subnormal from |g| = 3e-18 down (beta2 = 0.999): the change is that of the 64-bit formula for
+    every decade of eps that is accepted.  Off by the 16 + 4 roundings of the change, and by sqrt(2^-149 / (1 - beta2))
+    in the denominator."""
+    from renaissance_b200 import ops
+    g = torch.tensor([s * x for x in (1e-12, 1e-15, 1e-16, 1e-17, 3e-18, 1e-18, 1e-19, 1e-20, 1e-21, 1e-22, 1e-25) for s in (1, -1)],
+                     device="cuda").repeat(13)
+    least = least_eps(beta2, eight)
+    for eps in [least * 1.01] + [10.0 ** -k for k in range(4, 16) if 10.0 ** -k >= least]:
+        t = zero_states(g, eight)
+        eps = float(torch.tensor(eps, dtype=torch.float32))
+        ops.adamw_step(plan_of(t, 0.0, eight), one(0, torch.int32), 1.0, 0.9, beta2, eps)
+        want = -g.double() / (g.double().abs() + eps)
+        off = (t["w"][0].double() - want).abs()
+        rel = 20 * U + U / (1 - beta2) + 2.0 ** -74.5 / math.sqrt(1 - beta2) / eps      # 1 - beta2 is a float, too
+        assert (off <= rel * want.abs() + 1e-44).all(), (eps, float((off / want.abs()).max()))
+
+
+@pytest.mark.parametrize("x", [3e-17, 1e-18, 1e-19, 1e-20, 1e-21, 1e-23])
+def test_many_steps_with_tiny_gradients(x):
+    """Constant gradients at the smallest eps: every step changes the weight by lr g / (|g| + eps), whatever v loses."""
+    from renaissance_b200 import ops
+    beta2, steps = 0.999, 300
+    eps = float(torch.tensor(least_eps(beta2, False) * 1.01, dtype=torch.float32))
+    g = torch.full((260,), x, device="cuda")
+    g[1::2] *= -1
+    t = zero_states(g, False)
+    plan, n = plan_of(t, 0.0, False), one(0, torch.int32)
+    for _ in range(steps):
+        ops.adamw_step(plan, n, 1.0, 0.9, beta2, eps)
+    want = -steps * g.double() / (g.double().abs() + eps)
+    # a step: 16 roundings, 4 / (1 - 0.9) that m gathers, beta2's and 1 - beta2's own, 5 / (1 - beta2) that v gathers, half of
+    # that in its root, what v loses where it is subnormal; and a rounding of the weight, which is at most `want`
+    rel = (56 + steps) * U + (0.5 + 2.5) * U / (1 - beta2) + 2.0 ** -74.5 / math.sqrt(1 - beta2) / eps
+    off = (t["w"][0].double() - want).abs()
+    assert (off <= rel * want.abs()).all(), float((off / want.abs()).max())
+
+
+@pytest.mark.parametrize("x", [1e-12, 1e-16, 1e-17, 1e-18, 1e-20])
+def test_many_8bit_steps_with_tiny_gradients(x):
+    """8-bit v below 2^-116 is stored as zeros, which takes at most 2^-5 of the smallest eps from the denominator.  With one
+    gradient for all elements both states' blocks keep their largest element exactly (448 times the scale, to a
+    rounding): what is left is 2^-5 and the roundings of scales."""
+    from renaissance_b200 import ops
+    beta2, steps = 0.999, 100
+    eps = float(torch.tensor(least_eps(beta2, True) * 1.01, dtype=torch.float32))
+    g = torch.full((256,), x, device="cuda")
+    t = zero_states(g, True)
+    plan, n = plan_of(t, 0.0, True), one(0, torch.int32)
+    for _ in range(steps):
+        ops.adamw_step(plan, n, 1.0, 0.9, beta2, eps)
+    want = -steps * g.double() / (g.double().abs() + eps)
+    off = (t["w"][0].double() - want).abs()
+    assert (off <= 2.0 ** -5 * 1.01 * want.abs()).all(), float((off / want.abs()).max())

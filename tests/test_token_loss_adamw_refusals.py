@@ -159,6 +159,26 @@ def test_adamw_step_refuses(lib):
         assert step(plan=bad) == _lib.ERR_INVALID_ARGUMENT, field
 
 
+@pytest.mark.parametrize("bits,power", [(32, -55), (8, -53)])
+@pytest.mark.parametrize("beta2", [0.0, 0.99, 0.999, 0.999999])
+def test_adamw_step_refuses_an_eps_below_what_v_holds(lib, bits, power, beta2):
+    """Accepted values reach the next check (a misaligned image) and no launch."""
+    rc, plan = write(lib, [tensor()], bits=bits)
+    assert rc == 0
+    plan.image = 0x700008
+    least = 2.0 ** power / (1 - beta2) ** 0.5
+
+    def step(eps):
+        rc = lib.trb200_adamw_step(C.byref(plan), B, 0.1, None, 0.9, beta2, eps, None, None, 0, None)
+        assert rc == _lib.ERR_INVALID_ARGUMENT
+        return lib.trb200_last_error()
+
+    for eps in (least * 0.99, least / 10, 1e-30, 1.2e-38, 1e-45, 0.0, -least * 2, float("nan"), float("inf"), 1e38):
+        assert b"eps" in step(eps), eps
+    for eps in (least * 1.01, 1e-8, 1.0, 8e37):
+        assert b"image" in step(eps), eps
+
+
 # ------------------------------------------------------------------------------------------------ Python callers
 
 def test_python_callers_refuse_cpu_tensors_and_shapes():

@@ -579,8 +579,9 @@ int trb200_sgd_plain(float* weights, const float* grads, void* weights_half, int
  * 8-bit states are e4m3 codes (one byte an element) with a float scale per 128 elements
  * of a tensor, value = code * scale, m rounded to nearest and v stochastically (random
  * bits from Philox4x32-10 keyed by `seed`, counted by element, tensor and step); zeros
- * in codes and scales are zero states.  A non-finite gradient in a step that is not
- * skipped makes the 8-bit states of its 128 elements NaN.
+ * in codes and scales are zero states.  A non-finite g in a step that is not skipped
+ * makes the 8-bit states of its 128 elements NaN.  A finite one whose square overflows
+ * leaves v infinite in float (the element moves no more) and 2^127 in 8 bits.
  *
  * The plan: a description of the tensors that is written once on the host, copied to the
  * device by the caller, and used by every step.  Tensors may be of any size and of any

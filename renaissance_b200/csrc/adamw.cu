@@ -263,6 +263,14 @@ __device__ __forceinline__ float scale_of(float top) {
     return top < kSmallest ? 0.f : (top == INFINITY ? NAN : __fmul_rn(top, 1.0f / kE4m3Max));
 }
 
+// What an infinite v of a block with finite m is stored as: an infinity would take the block's other elements with it.
+// Half of the range, so that 448 times its scale does not overflow again: from there it decays like any other.
+constexpr float kHalfRange = 1.70141183e38f;    // 2^127
+__device__ __forceinline__ uint64_t at_most_half(uint64_t v) {
+    const float2 f = split(v);
+    return pair_of(fminf(f.x, kHalfRange), fminf(f.y, kHalfRange));
+}
+
 // A lane's elements of a scale block, 4 lane .. 4 lane + 3, and the block's scales.
 template <int GT>
 struct BlockLoad {
@@ -384,6 +392,10 @@ __device__ __forceinline__ void unit_8bit(const Tensor& t, int tensor, int64_t u
         }
         mt = warp_top(mt);
         vt = warp_top(vt);
+        if (vt == INFINITY && mt < INFINITY) {                  // seldom: the square of a finite gradient overflowed
+            v[k] = {at_most_half(v[k].a), at_most_half(v[k].b)};
+            vt = kHalfRange;
+        }
         if ((lane & 3) == 2 * k) top = mt;
         if ((lane & 3) == 2 * k + 1) top = vt;
     }

@@ -462,3 +462,47 @@ def test_many_8bit_steps_with_tiny_gradients(x):
     want = -steps * g.double() / (g.double().abs() + eps)
     off = (t["w"][0].double() - want).abs()
     assert (off <= 2.0 ** -5 * 1.01 * want.abs()).all(), float((off / want.abs()).max())
+
+
+# ------------------------------------------------------------------------------------------------ huge gradients
+
+@pytest.mark.parametrize("n", [256, 300])
+@pytest.mark.parametrize("x", [2e19, -1e20, 3e38])
+def test_a_finite_gradient_whose_square_overflows_spares_its_block(x, n):
+    """|g| > 1.8e19 has no square in floats.  8-bit v is stored as 2^127 there: nothing becomes NaN, the other elements'
+    first change is the formula's, v decays from the next step on."""
+    from renaissance_b200 import ops
+    g = torch.randn(n, generator=gen(1), device="cuda")
+    for at in (5, n - 1):
+        g[at] = x
+    t = zero_states(g.clone(), True, w=0.5)
+    plan, step = plan_of(t, 0.0, True), one(0, torch.int32)
+    ops.adamw_step(plan, step, LR)
+    tame = g.abs() < 1e3
+    want = 0.5 - LR * g.double() / (g.double().abs() + EPS)
+    # 1 - beta2 in floats is off by half a step of 0.999, U / 0.001 of v, half of that of the change
+    assert ((t["w"][0].double() - want).abs()[tame] <= 4 * U * 0.5 + (20 + 500) * U * LR).all()
+    assert (t["w"][0][~tame] == 0.5).all()                              # v is infinite in the update itself
+    value = lambda: t["v"][0].float().double() * t["vs"][0].repeat_interleave(128)[:n].double()
+    assert (t["m"][0].float().abs()[~tame] == 448).all()
+    last = value()
+    assert (last[~tame] >= 2.0 ** 127 * 0.92).all() and (last[~tame] <= 2.0 ** 127 * (1 + 8 * U)).all()     # one code below at most
+    g.fill_(1.0)
+    t["g"][0].fill_(1.0)
+    for _ in range(500):
+        ops.adamw_step(plan, step, LR)
+    assert t["w"][0].isfinite().all() and t["m"][0].float().isfinite().all() and t["v"][0].float().isfinite().all()
+    assert t["ms"][0].isfinite().all() and t["vs"][0].isfinite().all()
+    assert (value()[~tame] < 2.0 ** 127 * 0.9).all()                    # 0.999^500 = 0.61, stochastic codes of 1/8
+
+
+def test_8bit_states_with_a_non_finite_gradient_stay_nan():
+    """What saturates is the square of a finite gradient only."""
+    from renaissance_b200 import ops
+    for bad in (math.inf, -math.inf, math.nan):
+        g = torch.ones(384, device="cuda")
+        g[5], g[200] = bad, 1e20
+        t = zero_states(g, True)
+        ops.adamw_step(plan_of(t, 0.0, True), one(0, torch.int32), LR)
+        assert t["ms"][0][0].isnan() and t["vs"][0][0].isnan()
+        assert t["ms"][0][1:].isfinite().all() and t["vs"][0][1:].isfinite().all()

@@ -357,6 +357,8 @@ int trb200_policy_loss_fused(const void* logits, int64_t logits_stride, const in
  * x_p = beta * ((S_2p - S_2p+1) - (ref_2p - ref_2p+1)):
  *   loss_partial[p] = (-(1 - label_smoothing) log sigmoid(x_p) - label_smoothing log sigmoid(-x_p)) / pairs
  *   *loss = sum_p loss_partial[p],   dlogits = scaling * d loss / d logits
+ * A term with the factor 0 counts as 0, also where x_p is infinite (a label whose logit
+ * is minus infinity).
  * ref_logp [2 * pairs] is the reference policy's S (NULL: 0).  logp [rows] and seq_logp
  * [2 * pairs] are written too.  Rows in front of seq_starts[0] and behind
  * seq_starts[2 * pairs] - 1 do not count.  Bounds outside [0, rows] are clamped; bounds

@@ -794,7 +794,9 @@ preference_pairs(const double* logp, const float* row_sum, const int32_t* seq_st
         const double tail = exp(-fabs(x)), soft = log1p(tail);
         const double up = x >= 0 ? 1.0 / (1.0 + tail) : tail / (1.0 + tail);        // sigmoid(x)
         const double down = x >= 0 ? tail / (1.0 + tail) : 1.0 / (1.0 + tail);      // sigmoid(-x)
-        const double part = ((1.0 - smoothing) * (fmax(-x, 0.0) + soft) + smoothing * (fmax(x, 0.0) + soft)) / pairs;
+        // a term with the factor 0 is left out: an answer without chance (x infinite) would make it 0 * inf
+        const double part = ((smoothing < 1.0 ? (1.0 - smoothing) * (fmax(-x, 0.0) + soft) : 0.0) +
+                             (smoothing > 0.0 ? smoothing * (fmax(x, 0.0) + soft) : 0.0)) / pairs;
         loss_partial[p] = (float)(x == x ? part : x);
         s_pull = (float)(beta * (smoothing * up - (1.0 - smoothing) * down) / pairs * (double)scaling[0]);
     }

@@ -45,3 +45,34 @@ def test_kl_term_of_an_impossible_class_is_infinite(dtype, classes):
     out = ops.policy_loss_fused(z, y, logp.clamp_min(-5.0), torch.ones(4, device="cuda"), one(1.0), ref_logp=ref, kl_coef=0.1)
     assert math.isfinite(float(out["loss_partial"][0])) and (out["loss_partial"][1:] == math.inf).all()
     assert float(out["loss"]) == math.inf
+
+
+# ------------------------------------------------------------------------------------------------ preference loss
+
+@pytest.mark.parametrize("eps", [0.0, 0.1, 1.0])
+def test_preference_loss_of_an_impossible_answer(eps):
+    """A label whose logit is minus infinity makes S = -inf.  In the other answer x = +inf: the loss is eps * inf, without
+    smoothing 0; in the preferred one x = -inf and the loss is (1 - eps) * inf.  Gradients are finite, the other pair's
+    numbers the formula's."""
+    from renaissance_b200 import ops
+    z, y = rows_of(8, 300, torch.float32, seed=4), ints(8, 300)
+    logp, _ = stats64(z, y)
+    st = torch.tensor([0, 2, 4, 6, 8], dtype=torch.int32, device="cuda")
+    x = 0.5 * (logp[4:6].sum() - logp[6:8].sum())
+    soft = lambda v: torch.nn.functional.softplus(v)
+    other = ((1 - eps) * soft(-x) + eps * soft(x)) / 2
+    for row, sign in ((3, 1), (0, -1)):
+        w = z.clone()
+        w[row, int(y[row])] = -math.inf
+        out = ops.preference_loss_fused(w, y, st, None, one(1.0), 0.5, eps)
+        part = out["loss_partial"].tolist()
+        factor = eps if sign > 0 else 1 - eps
+        assert part[0] == (math.inf if factor else 0.0)
+        tol = 0.5 * float(logp_tol(logp, logp)[4:].sum()) + 8 * U
+        assert abs(part[1] - float(other)) <= tol
+        assert float(out["loss"]) == (math.inf if factor else part[1])
+        assert out["dlogits"].isfinite().all()
+        pull = 0.5 / 2 * (eps if sign > 0 else -(1 - eps))      # beta / pairs * (eps sigmoid(x) - (1 - eps) sigmoid(-x))
+        coef = torch.tensor([pull, pull, -pull, -pull], dtype=torch.float64, device="cuda")
+        lse = stats64(w, y)[1]
+        check_gradient(out["dlogits"][:4], w[:4], y[:4], coef, 2 * U * coef.abs(), U * (150 + 4 * lse.abs())[:4])

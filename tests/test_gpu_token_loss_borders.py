@@ -76,3 +76,86 @@ def test_preference_loss_of_an_impossible_answer(eps):
         coef = torch.tensor([pull, pull, -pull, -pull], dtype=torch.float64, device="cuda")
         lse = stats64(w, y)[1]
         check_gradient(out["dlogits"][:4], w[:4], y[:4], coef, 2 * U * coef.abs(), U * (150 + 4 * lse.abs())[:4])
+
+
+# ------------------------------------------------------------------------------------------------ large logits
+
+# shifts of a row's logits, and factors: maxima on both sides of 256 and of 2^100, ordinary rows among them
+MOVES = {torch.float16: [(0, 1), (245, 1), (-262, 1), (300, 1), (-1000, 1), (6e4, 1), (0, 100), (-6e4, 1), (0, 1), (250, 1)],
+         torch.bfloat16: [(0, 1), (245, 1), (-262, 1), (300, 1), (-1000, 1), (1e30, 1), (0, 1e30), (-1e30, 1), (0, 100), (250, 1),
+                          (3e38, 1), (-3e38, 1), (1e28, 1)]}
+MOVES[torch.float32] = MOVES[torch.bfloat16] + [(1e4, 1), (-1e4, 3)]
+FAR_CLASSES = [1, 9, 100, 200, 300, 450, 700, 1000, 1501, 2048, 2057, 5001, 16400, 33001, 70003, 140000]
+
+
+def far_rows(rows, classes, dtype, pad, skip, seed):
+    """(logits, labels, the same logits in 64 bits minus their row's maximum: the same distribution)."""
+    z = rows_of(rows, classes, dtype, pad, skip, seed)
+    y = ints(rows, classes, seed + 1)
+    for i in range(rows):
+        shift, factor = MOVES[dtype][i % len(MOVES[dtype])]
+        z[i] = (z[i].double() * factor + shift).to(dtype)
+        if factor > 1:
+            y[i] = int(z[i].float().argmax())               # any other class would have no chance at all
+    w = z.double()
+    return z, y, w - w.amax(1, keepdim=True)
+
+
+def spare_columns(rows, classes, dtype):
+    """A gradient buffer inside a wider one, at an odd alignment."""
+    flat = torch.full((1 + rows * (classes + 3) + 8,), 7.0, dtype=dtype, device="cuda")
+    return flat, torch.as_strided(flat, (rows, classes), (classes + 3, 1), 1)
+
+
+def kept_off(flat, d):
+    d.fill_(7.0)
+    return bool((flat == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", FAR_CLASSES)
+def test_policy_loss_with_large_logits(dtype, classes):
+    """A distribution does not change when all its logits move: loss and gradient to the tolerances of the logits minus
+    their maximum.  Up to 256 the 16-bit gradient's exponent is rounded at the logits' own size, 2^-16 of the result."""
+    from renaissance_b200 import ops
+    rows = 2 * len(MOVES[dtype])
+    for pad, skip, given in ((0, 0, False), (5, 1, True)):
+        z, y, zero = far_rows(rows, classes, dtype, pad, skip, 7)
+        logp, log_sum = stats64(zero, y)
+        moved = torch.where(floats(rows, 9) < 0, -0.1, 0.1).double()
+        old, ref = (logp - moved).float(), (logp + 0.2).float()
+        adv, w = floats(rows, 11), floats(rows, 12).abs() + 0.1
+        flat, d = spare_columns(rows, classes, dtype) if given else (None, None)
+        from test_gpu_token_losses import policy64
+        out = ops.policy_loss_fused(z, y, old, adv, one(64.0), 0.2, 0.28, ref, 0.05, w, dlogits=d)
+        part, want, coef, part_tol, t, coef_tol = policy64(zero, y, old, adv, ref, w, 0.2, 0.28, 0.05, 64.0)
+        near(out["logp"], want, t, "logp")
+        near(out["loss_partial"], part, part_tol, "loss_partial")
+        check_gradient(out["dlogits"], zero, y, coef, coef_tol, t + 2.0 ** -16 * (dtype != torch.float32))
+        got = ops.token_logprobs(z, y)
+        assert torch.equal(got["logp"], out["logp"])
+        near(got["lse"], log_sum + z.double().amax(1), t + U * (log_sum + z.double().amax(1)).abs(), "lse")
+        assert not given or (out["dlogits"].data_ptr() == d.data_ptr() and kept_off(flat, d))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", FAR_CLASSES)
+def test_preference_loss_with_large_logits(dtype, classes):
+    from renaissance_b200 import ops
+    from test_gpu_token_losses import preference64
+    rows = 2 * len(MOVES[dtype])
+    starts = [0, 3, rows // 2, rows // 2, rows - 1]
+    for pad, skip, given in ((0, 0, False), (5, 1, True)):
+        z, y, zero = far_rows(rows, classes, dtype, pad, skip, 5)
+        y[1] = -1
+        flat, d = spare_columns(rows, classes, dtype) if given else (None, None)
+        st = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        S = preference64(zero, y, starts, None, 0.1, 0.1, 64.0)[2]
+        ref = (S + floats(4, 3)).float()
+        out = ops.preference_loss_fused(z, y, st, ref, one(64.0), 0.1, 0.1, dlogits=d)
+        part, part_tol, S, S_tol, logp, t, coef, coef_tol = preference64(zero, y, starts, ref, 0.1, 0.1, 64.0)
+        near(out["logp"], logp, t, "logp")
+        near(out["seq_logp"], S, S_tol, "seq_logp")
+        near(out["loss_partial"], part, part_tol, "loss_partial")
+        check_gradient(out["dlogits"], zero, y, coef, coef_tol, t + 2.0 ** -16 * (dtype != torch.float32))
+        assert not given or kept_off(flat, d)

@@ -325,8 +325,11 @@ int trb200_softmax_ce_fused_dtype(const void* logits, int64_t logits_stride, con
 /* A row does not count if its label lies outside [0, classes), if its weight */
 /* is 0 or if all its logits are minus infinity: it adds nothing to the loss, */
 /* its row of dlogits is zero, and in the first two cases its logits are not  */
-/* read (they may hold anything).  rows may be 0.  Results are bitwise        */
-/* reproducible.                                                              */
+/* read (they may hold anything).  rows may be 0.  A call that is repeated on */
+/* the same buffers gives the same bits.  A row's logp is the same number in  */
+/* every batch and in all three operators where its address modulo 16 bytes   */
+/* is the same (strides of whole 16 bytes keep it); elsewhere its sum is      */
+/* taken in another order, and logp may differ in its last bits.              */
 /* ------------------------------------------------------------------------- */
 
 /* logp[i] = z_i[y_i] - lse[i], lse[i] = log(sum_c exp(z_i[c])): what the policy that

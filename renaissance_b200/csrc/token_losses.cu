@@ -619,7 +619,10 @@ rows_short(Rows<DT> r, P p) {
 // ---------------------------------------------------------------- longer rows: streamed
 // A row is cut into parts by its length alone, up to kMaxParts of them; a cluster of C blocks shares it, `per_block`
 // parts each.  Every part has its own maximum and sum, and they are merged in one order whatever C is: a row's
-// log-probability is the same number in every batch and in every operator.
+// log-probability is the same number in every batch and in every operator, as long as the row's address modulo 16 bytes
+// is the same.  Vectors start at aligned addresses, so that a row that moves to another alignment (odd class counts or
+// strides) is summed in another order: of 200 rows of 1001, 2047 or 50021 classes 4 to 10 then came out different, by
+// 2e-6 at most.
 //
 // The gradient reads the row again.  The blocks that are resident at once (six of 256 threads an SM) hold 64 KB of logits
 // each, 57 MB in all, so that the second read comes from L2 (4096 x 32000 bfloat16: 269 MB are read from HBM, 262 MB of
@@ -949,7 +952,7 @@ Rows<DT> rows_of(const LogitArgs& a) {
     return {static_cast<const T*>(a.logits), a.logits_stride, static_cast<T*>(a.dlogits), a.dlogits_stride, a.labels, a.rows, a.classes};
 }
 
-// One kernel over the rows.  Which one goes by their length alone, as do the sums in it.
+// One kernel over the rows.  Which one goes by their length alone, as do the sums in it but for the row's alignment.
 template <int DT, class P>
 int launch_rows(const Rows<DT>& r, const P& p, cudaStream_t s, const char* who) {
     const int nvec = r.classes / Logit<DT>::kVec;

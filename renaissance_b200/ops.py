@@ -693,7 +693,9 @@ def _gradient_rows(dlogits, logits, n, k):
 def token_logprobs(logits, labels, stream=None):
     """Log-probability of each row's label and the row's log-sum-exp: dict(logp, lse), float [rows].  logits [rows,
     classes] half, bfloat16 or float, labels int32.  A label outside [0, classes) gives 0 and 0 and its row is not
-    read; a row of minus infinities gives -inf and -inf."""
+    read; a row of minus infinities gives -inf and -inf.  A row's logp is the same number here and in the losses, in any
+    batch, where the row's address modulo 16 bytes is the same (keep the row stride a multiple of 16 bytes if rows move
+    between batches); elsewhere it may differ in its last bits."""
     n, k, stride = _logit_rows(logits, "logits")
     dev = logits.device
     labels_p = _vector(labels, n, torch.int32, "labels", dev)

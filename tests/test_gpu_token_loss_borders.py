@@ -159,3 +159,40 @@ def test_preference_loss_with_large_logits(dtype, classes):
         near(out["loss_partial"], part, part_tol, "loss_partial")
         check_gradient(out["dlogits"], zero, y, coef, coef_tol, t + 2.0 ** -16 * (dtype != torch.float32))
         assert not given or kept_off(flat, d)
+
+
+# ------------------------------------------------------------------------------------------------ rows that move
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [9, 100, 777, 1001, 2047, 2049, 5001, 33001, 50021])
+def test_a_row_that_moves_keeps_its_logp_to_its_alignment(dtype, classes):
+    """The same rows in another order, at other strides and offsets: bit for bit the same where a row's address modulo 16
+    bytes is, a ratio of exactly 1 in the loss among it; elsewhere within twice what one sum may be off by."""
+    from renaissance_b200 import ops
+    rows, item = 48, torch.finfo(dtype).bits // 8
+    wide = 16 // item
+    z, y = rows_of(rows, classes, dtype, seed=3), ints(rows, classes)
+    first = ops.token_logprobs(z, y)
+    where = lambda t: (t.data_ptr() + torch.arange(rows, device="cuda") * t.stride(0) * item) % 16
+    tol = 2 * logp_tol(*stats64(z, y))
+    order = torch.randperm(rows, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    moves = 0
+    for pad, skip, perm in ((0, 0, order), (-classes % wide, 0, order), (5, 1, order), (0, wide, order), (wide, 3, torch.arange(rows, device="cuda"))):
+        w = rows_of(rows, classes, dtype, pad, skip)
+        w.copy_(z[perm])
+        got = ops.token_logprobs(w, y[perm])
+        same = where(w) == where(z)[perm]
+        moves += int((~same).sum())
+        for k in ("logp", "lse"):
+            assert torch.equal(got[k][same], first[k][perm][same])
+            assert ((got[k].double() - first[k][perm].double()).abs() <= tol[perm]).all()
+        adv = floats(rows, 5)
+        out = ops.policy_loss_fused(w, y[perm], first["logp"][perm], adv, one(1.0), weights=torch.ones(rows, device="cuda"))
+        assert torch.equal(out["logp"], got["logp"])
+        assert torch.equal(out["loss_partial"][same], -adv[same])
+    # an aligned stride keeps every row's alignment, wherever it goes
+    a, b = (rows_of(rows, classes, dtype, -classes % wide, s) for s in (0, 2 * wide))
+    a.copy_(z)
+    b.copy_(z[order])
+    assert torch.equal(ops.token_logprobs(b, y[order])["logp"], ops.token_logprobs(a, y)["logp"][order])
+    assert moves > 0

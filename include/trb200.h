@@ -319,9 +319,10 @@ int trb200_softmax_ce_fused_dtype(const void* logits, int64_t logits_stride, con
 /* Losses over the log-probabilities of chosen classes, beside softmax-CE.    */
 /* The reference has no counterpart.  `logits` and `dlogits` are rows of      */
 /* `classes` elements of `dtype` (half, bfloat16 or float) with row strides   */
-/* in elements, aligned to their element only; dlogits must not overlap       */
-/* logits (not even in the padding between rows).  `scaling` is the loss scale */
-/* (device scalar): it multiplies dlogits, not the loss.                      */
+/* in elements.  They and all arrays are aligned to their element (a call with */
+/* one that is not is refused); no more than that is needed.  dlogits must not */
+/* overlap logits (not even in the padding between rows).  `scaling` is the   */
+/* loss scale (device scalar): it multiplies dlogits, not the loss.           */
 /* A row does not count if its label lies outside [0, classes), if its weight */
 /* is 0 or if all its logits are minus infinity: it adds nothing to the loss, */
 /* its row of dlogits is zero, and in the first two cases its logits are not  */

@@ -635,6 +635,8 @@ extern "C" int trb200_adamw_step(const trb200_adamw_plan* plan, int32_t* step, f
                                  double beta2, float eps, const float* scaling, const int32_t* skip_flag, uint64_t seed,
                                  void* stream) {
     TRB_REQUIRE(plan && plan->image && step, TRB200_ERR_INVALID_ARGUMENT, "adamw_step: null pointer");
+    TRB_REQUIRE(trb::aligned4(step, lr_dev, scaling, skip_flag), TRB200_ERR_INVALID_ARGUMENT,
+                "adamw_step: step, lr_dev, scaling and skip_flag must be aligned to 4 bytes");
     TRB_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, TRB200_ERR_INVALID_ARGUMENT,
                 "adamw_step: beta1 and beta2 must lie in [0, 1)");
     TRB_REQUIRE(std::isfinite(lr), TRB200_ERR_INVALID_ARGUMENT, "adamw_step: lr must be finite");

@@ -22,6 +22,10 @@ inline cudaEvent_t as_event(void* e) { return static_cast<cudaEvent_t>(e); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether all of the given pointers (null ones too) are aligned to 4-byte elements.
+template <class... P>
+inline bool aligned4(const P*... p) { return ((... | reinterpret_cast<uintptr_t>(p)) & 3u) == 0; }
+
 inline int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 // Number of SMs of the current device (cached per device).

@@ -1006,6 +1006,8 @@ extern "C" int trb200_token_logp(const void* logits, int64_t logits_stride, cons
     if (rc != TRB200_OK) return rc;
     if (rows == 0) return TRB200_OK;
     TRB_REQUIRE(logp, TRB200_ERR_INVALID_ARGUMENT, "token_logp: null pointer");
+    TRB_REQUIRE(trb::aligned4(labels, logp, lse), TRB200_ERR_INVALID_ARGUMENT,
+                "token_logp: labels, logp and lse must be aligned to 4 bytes");
     const trb::LogpRows p{logp, lse};
 #define TRB_LAUNCH(DT) return trb::launch_rows<DT>(trb::rows_of<DT>(a), p, trb::as_stream(stream), "token_logp")
     TRB_BY_DTYPE(dtype, TRB_LAUNCH);
@@ -1027,6 +1029,8 @@ extern "C" int trb200_policy_loss_fused(const void* logits, int64_t logits_strid
     TRB_REQUIRE(ref_logp || kl_coef == 0.f, TRB200_ERR_INVALID_ARGUMENT, "policy_loss: a KL term needs ref_logp");
     TRB_REQUIRE(rows == 0 || (old_logp && advantages && logp && loss_partial), TRB200_ERR_INVALID_ARGUMENT,
                 "policy_loss: null pointer");
+    TRB_REQUIRE(trb::aligned4(actions, old_logp, ref_logp, advantages, weights, scaling, logp, loss_partial, loss),
+                TRB200_ERR_INVALID_ARGUMENT, "policy_loss: arrays of 4-byte elements must be aligned to them");
     const trb::PolicyArgs p{old_logp, kl_coef != 0.f ? ref_logp : nullptr, advantages, weights, scaling, 1.0f - clip_low,
                             1.0f + clip_high, kl_coef, rows ? 1.0f / (float)rows : 0.f};
     if (rows > 0) {
@@ -1058,6 +1062,8 @@ extern "C" int trb200_preference_loss_fused(const void* logits, int64_t logits_s
     TRB_REQUIRE(pairs > 0 && pairs <= (1 << 29), TRB200_ERR_INVALID_ARGUMENT, "preference_loss: bad number of pairs (%d)", pairs);
     TRB_REQUIRE(seq_starts && scaling && seq_logp && loss_partial && loss && (rows == 0 || logp),
                 TRB200_ERR_INVALID_ARGUMENT, "preference_loss: null pointer");
+    TRB_REQUIRE(trb::aligned4(labels, seq_starts, ref_logp, scaling, logp, seq_logp, loss_partial, loss),
+                TRB200_ERR_INVALID_ARGUMENT, "preference_loss: arrays of 4-byte elements must be aligned to them");
     TRB_REQUIRE(std::isfinite(beta) && label_smoothing >= 0.0 && label_smoothing <= 1.0, TRB200_ERR_INVALID_ARGUMENT,
                 "preference_loss: beta must be finite and label_smoothing lie in [0, 1]");
     TRB_REQUIRE(rows == 0 || (workspace && workspace_bytes >= trb200_preference_loss_workspace_bytes(rows) &&

@@ -75,6 +75,18 @@ def test_preference_loss_needs_its_workspace(lib):
     assert preference(lib, ws=E + 4) == _lib.ERR_WORKSPACE
 
 
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_arrays_of_four_byte_elements_have_to_be_aligned(lib, off):
+    """A misaligned address would end in a fault of the GPU: refused before any launch."""
+    calls = ((logp, "token_logp", ("labels", "out", "lse")),
+             (policy, "policy_loss", ("y", "old", "ref", "adv", "w", "sc", "lp", "part", "loss")),
+             (preference, "preference_loss", ("y", "starts", "ref", "sc", "lp", "seq", "part", "loss")))
+    for call, name, fields in calls:
+        for field in fields:
+            assert call(lib, **{field: B + off}) == _lib.ERR_INVALID_ARGUMENT, field
+            assert name.encode() in lib.trb200_last_error() and b"aligned" in lib.trb200_last_error(), field
+
+
 # ------------------------------------------------------------------------------------------------ AdamW
 
 def tensor(n=1000, at=0x100000, **kw):
@@ -177,6 +189,17 @@ def test_adamw_step_refuses_an_eps_below_what_v_holds(lib, bits, power, beta2):
         assert b"eps" in step(eps), eps
     for eps in (least * 1.01, 1e-8, 1.0, 8e37):
         assert b"image" in step(eps), eps
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("field", range(4))
+def test_adamw_step_refuses_misaligned_scalars(lib, field, off):
+    rc, plan = write(lib, [tensor()])
+    assert rc == 0
+    plan.image = 0x700000
+    step, lr, scaling, skip = ((B + off if i == field else B) for i in range(4))
+    assert lib.trb200_adamw_step(C.byref(plan), step, 0.1, lr, 0.9, 0.999, 1e-8, scaling, skip, 0, None) == _lib.ERR_INVALID_ARGUMENT
+    assert b"aligned to 4 bytes" in lib.trb200_last_error()
 
 
 # ------------------------------------------------------------------------------------------------ Python callers

@@ -316,21 +316,22 @@ int trb200_softmax_ce_fused_dtype(const void* logits, int64_t logits_stride, con
                                   int32_t batch, int32_t classes, int32_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------- */
-/* Losses over the log-probabilities of chosen classes, beside softmax-CE.    */
-/* The reference has no counterpart.  `logits` and `dlogits` are rows of      */
-/* `classes` elements of `dtype` (half, bfloat16 or float) with row strides   */
-/* in elements.  They and all arrays are aligned to their element (a call with */
-/* one that is not is refused); no more than that is needed.  dlogits must not */
-/* overlap logits (not even in the padding between rows).  `scaling` is the   */
-/* loss scale (device scalar): it multiplies dlogits, not the loss.           */
-/* A row does not count if its label lies outside [0, classes), if its weight */
-/* is 0 or if all its logits are minus infinity: it adds nothing to the loss, */
-/* its row of dlogits is zero, and in the first two cases its logits are not  */
-/* read (they may hold anything).  rows may be 0.  A call that is repeated on */
-/* the same buffers gives the same bits.  A row's logp is the same number in  */
-/* every batch and in all three operators where its address modulo 16 bytes   */
-/* is the same (strides of whole 16 bytes keep it); elsewhere its sum is      */
-/* taken in another order, and logp may differ in its last bits.              */
+/* Losses over the log-probabilities of chosen classes, beside softmax-CE. The */
+/* reference has no counterpart.  `logits` and `dlogits` are rows of `classes` */
+/* elements of `dtype` (half, bfloat16 or float) with row strides in elements. */
+/* They and all arrays are aligned to their element (a call with one that is   */
+/* not is refused); no more than that is needed.  dlogits must not overlap     */
+/* logits (not even in the padding between rows).  `scaling` is the loss scale */
+/* (device scalar): it multiplies dlogits, not the loss. A row does not count  */
+/* if its label lies outside [0, classes), if its weight is 0 or if all its    */
+/* logits are minus infinity: it adds nothing to the loss, its row of dlogits  */
+/* is zero, and in the first two cases its logits are not read (they may hold  */
+/* anything).  A NaN or +infinity among the logits of a row that counts makes  */
+/* its numbers NaN.  rows may be 0.  A call that is repeated on the same       */
+/* buffers gives the same bits.  A row's logp is the same number in every      */
+/* batch and in all three operators where its address modulo 16 bytes is the   */
+/* same (strides of whole 16 bytes keep it); elsewhere its sum is taken in     */
+/* another order, and logp may differ in its last bits.                        */
 /* ------------------------------------------------------------------------- */
 
 /* logp[i] = z_i[y_i] - lse[i], lse[i] = log(sum_c exp(z_i[c])): what the policy that

@@ -56,6 +56,15 @@ void note_launch();
         if (!(cond)) return ::trb::fail(code, __VA_ARGS__); \
     } while (0)
 
+#ifdef __CUDACC__
+// 2^x to 2^-22; results below 2^-126 are 0
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+#endif
+
 // 16-bit storage types.  The kernels are written once over these helpers: BF16 = false is IEEE half (the
 // reference's AMP dtype), BF16 = true is bfloat16.  All arithmetic is float either way.
 #ifdef __CUDACC__

@@ -319,19 +319,41 @@ __device__ __forceinline__ float exp_excess(float x, float more) {
     return x * x * p;
 }
 
-// Weighted loss of a row and scaling * its derivative with respect to logp.  The ratio is taken from logp as it is stored,
-// a float (2^-24 of |logp|, 5e-7 for 8 to 16), not from more digits of it: old_logp is such a float of token_logp(), and only
-// so a policy that has not moved has a ratio of exactly 1.
-__device__ __forceinline__ void policy_row(const PolicyArgs& a, const PolicyIn& in, float logp, float& loss, float& coef) {
+// a - b and what its rounding cut off
+__device__ __forceinline__ float minus_with_rest(float a, float b, float& rest) {
+    const float d = a - b, back = d - a;
+    rest = (a - (d - back)) - (b + back);
+    return d;
+}
+
+// log-probability of the label with logit zy minus old, which is near it, to 2^-24: ((zy - m) - old) - log s with what the two
+// differences cut off, and with s = 2^e f, f in [0.75, 1.5): log s = e ln 2 + log f.  ln 2 is in two floats, the first short
+// enough for e ln 2 to be exact.
+__device__ __forceinline__ float moved_since(float old, float zy, MaxSum a) {
+    constexpr float kLn2Hi = 0.693145751953125f, kLn2Lo = 1.42860682e-6f;
+    const int e = (__float_as_int(a.s) - 0x3f400000) >> 23;
+    const float log_f = logf(a.s * __int_as_float((127 - e) << 23)), p = (float)e;
+    float r1, r2;
+    const float d = minus_with_rest(minus_with_rest(zy, a.m, r1), old, r2);
+    return (fmaf(-p, kLn2Hi, d) - log_f) + (r1 + fmaf(-p, kLn2Lo, r2));
+}
+
+// Weighted loss of a row and scaling * its derivative with respect to logp.  The stored logp is off by half a step of a float
+// (5e-7 for 8 to 16), which the ratio would take over.  Where old_logp is that very float the policy has not moved, and the
+// ratio is exactly 1.
+__device__ __forceinline__ void policy_row(const PolicyArgs& a, const PolicyIn& in, float logp, float zy, MaxSum stats, float& loss,
+                                           float& coef) {
     const float adv = in.advantage;
-    const float ratio = expf(logp - in.old_logp);
+    float moved = logp - in.old_logp;
+    if (moved != 0.f && fabsf(moved) < INFINITY) moved = moved_since(in.old_logp, zy, stats);
+    const float ratio = expf(moved);
     const float kept = ratio * adv;
     const float cut = fminf(fmaxf(ratio, a.low), a.high) * adv;
     float l, g;
     if (kept <= cut) { l = -kept; g = -kept; }
     else { l = kept > cut ? -cut : NAN; g = kept > cut ? 0.f : NAN; }     // unordered: a NaN stays one
     if (a.ref_logp) {
-        const float gap = in.ref_logp - logp;
+        const float gap = in.ref_logp - logp;                   // of the floats: 0 where the reference's is the same one
         const float more = expm1f(gap);                         // no cancellation next to gap = 0
         l += a.kl_coef * exp_excess(gap, more);
         g -= a.kl_coef * more;
@@ -392,7 +414,7 @@ struct PolicyRows {
         float lp = 0.f, loss = 0.f, coef = 0.f;
         if (a.s != 0.f) {
             lp = label_logp(zy, a);
-            policy_row(p, x, lp, loss, coef);
+            policy_row(p, x, lp, zy, a, loss, coef);
         }
         if (write) {
             logp[row] = lp;

@@ -196,3 +196,34 @@ def test_a_row_that_moves_keeps_its_logp_to_its_alignment(dtype, classes):
     b.copy_(z[order])
     assert torch.equal(ops.token_logprobs(b, y[order])["logp"], ops.token_logprobs(a, y)["logp"][order])
     assert moves > 0
+
+
+# ------------------------------------------------------------------------------------------------ digits of the ratio
+
+@pytest.mark.parametrize("classes", [16, 1000, 5001])
+def test_ratio_has_more_digits_than_the_stored_logp(classes):
+    """Five classes near the maximum, the chosen one 100 below it, nothing else: log s is good to 10 u (five exponentials of
+    4 u, nine additions and merges that change nothing but add to one another), the float that logp is stored as to 64 u.
+    Of the ratio: 10 u, 1 u for log s and for the difference, 4 u for its exponential, 3 u of products."""
+    from renaissance_b200 import ops
+    rows = 256
+    z = torch.full((rows, classes), -math.inf, device="cuda")
+    z[:, :5] = 3.0 + rows_of(rows, 5, torch.float32, seed=1, spread=0.3)
+    z[:, 9] = -97.0 + floats(rows, 2)
+    y = torch.full((rows,), 9, dtype=torch.int32, device="cuda")
+    logp, _ = stats64(z, y)
+    old = (logp + 0.1 * floats(rows, 3).double()).float()
+    adv, w = -torch.ones(rows, device="cuda"), torch.ones(rows, device="cuda")         # no upper bound for a loss
+    out = ops.policy_loss_fused(z, y, old, adv, one(1.0), 1.0, 10.0, weights=w)
+    ratio = torch.exp(logp - old.double())
+    near(out["loss_partial"], ratio, 20 * U * ratio, "ratio")
+    # a policy that has not moved
+    out = ops.policy_loss_fused(z, y, out["logp"], adv, one(1.0), 1.0, 10.0, weights=w)
+    assert (out["loss_partial"] == 1).all()
+    z[3, 9] = z[4, 7] = -math.inf                           # impossible now as it was then: no ratio; z[4] is as before
+    old = ops.token_logprobs(z, y)["logp"]
+    out = ops.policy_loss_fused(z, y, old, adv, one(1.0), 1.0, 10.0, weights=w)
+    assert out["loss_partial"][3].isnan() and (out["loss_partial"][4:] == 1).all()
+    z[5, 2], z[6, 1] = math.nan, math.inf
+    out = ops.policy_loss_fused(z, y, torch.full_like(old, -100.0), adv, one(1.0), 1.0, 10.0, weights=w)
+    assert out["loss_partial"][5:7].isnan().all() and out["loss_partial"][7:].isfinite().all()

@@ -14,10 +14,11 @@
 // becomes 0, which would make the update m / eps.
 //
 // Bound by HBM: 8 B of weight, the gradient, the copy and 16 B (float) or 4.125 B (8-bit) of state per element.  Float
-// states reach it: 138 M elements in 653 us, 0.97 of the copy bandwidth.  8-bit ones come near (488 us, 0.79; 25.6 M
-// elements with 16-bit gradients 87 us, 0.72): their 55 instructions an element (decoding, the update, the largest
-// magnitude of a block, random bits, encoding) take about as long as the bytes do, so that loads have to be on their way
-// all the time (asynchronous copies, three units ahead a warp) and pairs of floats go through the packed instructions.
+// states reach it: 138 M elements in 652 us, 0.97 of the copy bandwidth.  8-bit ones come near (480 us, 0.80; 25.6 M
+// elements with 16-bit gradients 88 us, 0.72): their 61 instructions an element (decoding, the update, the largest
+// magnitude of a block, random bits, encoding) take 64 % of the issue slots, and 24 warps an SM do not hide all of a unit's
+// chain of them.  So loads have to be on their way all the time (asynchronous copies, three units ahead a warp), and pairs of
+// floats go through the packed instructions.
 #include "chained.cuh"
 #include "common.cuh"
 #include "packed.cuh"

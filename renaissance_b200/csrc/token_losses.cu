@@ -515,7 +515,7 @@ __device__ __forceinline__ void row_gradient(const typename Logit<DT>::T* z, typ
 // ---------------------------------------------------------------- short rows: in registers
 // G lanes of a warp share a row, K vectors each; what a row costs beside its elements (setting up, merging, the loss
 // itself) is paid once for the 32 / G rows of the warp: log-probabilities of 65536 rows of 64 bfloat16 classes take 6.4 us
-// with 8 lanes a row, 22.0 us with 32.  65536 x 1000 take 27.5 us (0.73 of the copy bandwidth), the policy loss 64.8 us.
+// with 8 lanes a row, 22.0 us with 32.  65536 x 1000 take 27.3 us (0.74 of the copy bandwidth), the policy loss 70 us.
 // Up to 2048 classes: 16383 x 1100 floats take 15.1 us (policy 39.6) here and 21.2 us (40.5) streamed.  Beyond, 16 bits,
 // 16384 x 4096: 23.9 us against 28.0, but the policy loss 59 us against 52.4, and all operators have to take the same
 // kernel for a length (see launch_rows).
@@ -648,9 +648,9 @@ rows_short(Rows<DT> r, P p) {
 // logits).  Shorter rows get smaller blocks: what a row costs beside its elements is paid by every warp of its block
 // (log-probabilities, 16384 rows: 2056 classes 25.1 us with 64 threads, 56.9 us with 256; 4096 classes 28.0 and 60.1 us).
 //
-// Log-probabilities of 6000 x 50021: 91 us, 0.81 of the copy bandwidth.  Policy loss: 4096 x 32000, a quarter of the rows
-// masked, 86 us, 0.82; 8192 x 131072, a tenth masked, 756 us, 0.83.  At 4096 x 32000 with every row counting, 11.4
-// instructions a logit take 51 % of the issue slots and the exponentials 75 % of their unit; warps wait for loads and for
+// Log-probabilities of 6000 x 50021: 88 us, 0.83 of the copy bandwidth.  Policy loss: 4096 x 32000, a quarter of the rows
+// masked, 85 us, 0.83; 8192 x 131072, a tenth masked, 750 us, 0.83.  At 4096 x 32000 with every row counting, 11.7
+// instructions a logit take 51 % of the issue slots and the exponentials 72 % of their unit; warps wait for loads and for
 // the block's barriers.  In a loop the GPU runs into its power limit at 8192 x 131072 (1000 W, 1.6 GHz).
 constexpr int kStreamThreads = 1536;         // of an SM, in blocks of 64, 128 or 256
 constexpr int kMaxParts = 8;
@@ -870,7 +870,7 @@ partial_loss_sum(const float* partial, int n, float* loss) {
 
 // Second pass of the preference loss: every row's maximum, sum and coef are known, nothing is left to wait for.  G threads
 // a row, or G = all of the block's for each of the `parts` of a long one; a thread's vectors in batches of four loads.
-// The first block also adds up the loss.  Bound by HBM: 4096 x 32000 bfloat16 take 81 us under the profiler, 473 MB at 71 %
+// The first block also adds up the loss.  Bound by HBM: 4096 x 32000 bfloat16 take 82 us under the profiler, 472 MB at 70 %
 // of the DRAM's peak.  Groups of threads against a block a row (whole preference loss): 65536 x 64 31 us against 166 us,
 // 16384 x 4096 78 us against 102 us.
 constexpr int kSlopeThreads = 256;

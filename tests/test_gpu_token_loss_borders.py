@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_token_losses import DTYPES, U, check_gradient, floats, ints, logp_tol, near, one, rows_of, stats64
+from test_gpu_token_losses import (DTYPES, U, check_gradient, floats, ints, logp_tol, near, one, policy64, preference64, rows_of,
+                                   stats64)
 
 pytestmark = pytest.mark.gpu
 
@@ -126,7 +127,6 @@ def test_policy_loss_with_large_logits(dtype, classes):
         old, ref = (logp - moved).float(), (logp + 0.2).float()
         adv, w = floats(rows, 11), floats(rows, 12).abs() + 0.1
         flat, d = spare_columns(rows, classes, dtype) if given else (None, None)
-        from test_gpu_token_losses import policy64
         out = ops.policy_loss_fused(z, y, old, adv, one(64.0), 0.2, 0.28, ref, 0.05, w, dlogits=d)
         part, want, coef, part_tol, t, coef_tol = policy64(zero, y, old, adv, ref, w, 0.2, 0.28, 0.05, 64.0)
         near(out["logp"], want, t, "logp")
@@ -142,7 +142,6 @@ def test_policy_loss_with_large_logits(dtype, classes):
 @pytest.mark.parametrize("classes", FAR_CLASSES)
 def test_preference_loss_with_large_logits(dtype, classes):
     from renaissance_b200 import ops
-    from test_gpu_token_losses import preference64
     rows = 2 * len(MOVES[dtype])
     starts = [0, 3, rows // 2, rows // 2, rows - 1]
     for pad, skip, given in ((0, 0, False), (5, 1, True)):
